@@ -396,6 +396,33 @@ int sana_dwconv_glu_amax(const void* u, const void* halo_top, const void* halo_b
                          const void* bias, void* out, int64_t rows, int64_t W, int64_t H, int64_t row0,
                          int64_t hid, float* amax_out, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * 8-bit projections with one power-of-two scale for each block of 128 elements along K.  Upstream has no FP8
+ * arithmetic of its own (its FP8 goes through Transformer Engine's te.Linear); these entry points replace the same
+ * nn.Linear / 1x1 Conv2d calls as sana_gemm with both operands in E4M3.
+ *
+ * Format: codes [rows, K] of one byte, row stride K; scales as E8M0 bytes (exponent + 127), entry
+ * (r / block_rows) * ldsf + k / 128, block_rows 1 (usual for activations) or 128 (usual for weights).
+ *   e = the least integer with amax <= 448 * 2^e, at least -126; amax = the largest magnitude of the block's finite
+ *   elements;  code = E4M3(x * 2^-e), round to nearest even;  an infinity or NaN becomes the code of NaN and does not
+ *   enter amax.
+ *
+ * sana_fp8_quantize: x [rows, K] of `dtype` (row stride ld, rows 16-byte aligned) -> q, sf.  K % 16 == 0.  One launch,
+ *   nothing is read back.
+ * sana_gemm_fp8: out [M, N] bf16 = epilogue(A @ W^T) with the sana_gemm epilogue;
+ *   A @ W^T = sum over blocks of 2^(ea + ew) * (product of the codes), fp32 accumulation.  K % 16 == 0, N % 8 == 0.
+ *   Scale rows must be 4-byte aligned, ldsfa / ldsfw multiples of 4, and each row readable up to the next multiple
+ *   of 4 blocks (what lies there is not used).  tcgen05.mma kind::mxf8f6f4, which applies the scales itself;
+ *   M >= 2048: CTA pairs on 256 x 256 tiles, else one CTA on 128 x 128 tiles (sana_gemm_set_variant overrides).
+ */
+int sana_fp8_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t ldsf, int64_t rows, int64_t K,
+                      int block_rows, int dtype, void* stream);
+int sana_gemm_fp8(const void* Aq, const void* sfa, int64_t ldsfa, int a_block_rows, const void* Wq, const void* sfw,
+                  int64_t ldsfw, int w_block_rows, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                  const sana_gemm_epilogue* ep, void* stream);
+/* Soft-error word of the tensor-core kernels of sana_gemm_fp8 (as sana_gemm_take_device_status). */
+int sana_gemm_fp8_take_device_status(int* status_out);
+
 /* Soft-error word of the tensor-core GEMM: its bounded waits record a code here instead of
  * spinning forever.  Returns 0 when no wait ever timed out on the current device since the
  * last call (host-synchronising: use in tests / after a failure, not per step). */

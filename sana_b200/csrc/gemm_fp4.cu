@@ -47,17 +47,6 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* gsrc, u
                : "memory");
 }
 
-// 32 rows x 16 bytes, rows contiguous: 8-row groups 128 bytes apart, no swizzle
-__device__ __forceinline__ uint64_t make_sf_desc(uint32_t saddr) {
-  const uint32_t lo = (saddr >> 4) & 0x3FFFu;
-  const uint32_t hi = (128u >> 4) | (1u << 14);
-  return ((uint64_t)hi << 32) | lo;
-}
-
-__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint64_t sdesc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-
 __device__ __forceinline__ void umma_nvfp4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
                                            uint32_t sfb, uint32_t accumulate) {
   asm volatile(
@@ -294,13 +283,6 @@ static_assert(P4_STAGE_BYTES % 1024 == 0, "stage bases must stay 1024-byte align
 static_assert(P4_SF_COL0 + P4_STAGES * P4_SF_COLS <= 512, "tensor memory budget");
 static_assert(16 * P4_STAGES + 40 + 8 * P4_EPI_WARPS + 8 * P4_STAGES <= P4_CTRL_BYTES, "control block too small");
 
-__device__ __forceinline__ void tmem_cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-// arrive (once, on this CTA's barrier) when every tcgen05 operation this thread has issued so far is complete
-__device__ __forceinline__ void tc_commit_pair_local(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void umma_nvfp4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
                                                 uint32_t sfb, uint32_t accumulate) {
   asm volatile(

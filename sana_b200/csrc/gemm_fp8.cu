@@ -1,0 +1,762 @@
+// 8-bit projection with one power-of-two scale for each block of 128 along K:
+//
+//   out[m][n] = epilogue( sum_kb 2^(ea[m][kb] + ew[n][kb]) * sum_{k in block kb} a[m][k] w[n][k] )
+//
+// a, w are E4M3 codes (K-major), ea / ew the exponents, stored as E8M0 bytes (exponent + 127) in a plain row-major
+// matrix [ceil(rows / block_rows), blocks], block_rows 1 (activations) or 128 (weights).  A power of two costs the
+// quantiser no rounding of its own (x * 2^-e is exact) and is what the tensor core applies itself
+// (tcgen05.mma kind::mxf8f6f4 takes one E8M0 scale for each row and 32 K elements): the partial sums of a block never
+// leave tensor memory, where a general fp32 scale would have to read them back after every 128 elements.
+//
+// The tensor core reads scales from tensor memory, as 4-column tiles of 128 rows x 4 bytes (byte b = scale b of the
+// row; the instruction names the byte), filled from 512-byte shared-memory tiles [row % 32][row / 32][b].  One byte
+// serves a whole stage here (K = 128 = four instructions), so a tile feeds four stages.  A warp of its own builds the
+// tiles from the plain scale matrix - one 32-bit load per row gives the bytes of four stages - and copies them with
+// tcgen05.cp, one tile ahead of the MMAs: weights are read in the layout they are stored in, nothing is repacked.
+#include <cuda_fp8.h>
+
+#include "tc_common.cuh"
+
+namespace sana {
+
+__device__ int g_fp8_status = 0;
+
+constexpr int F8_BK = 128;                       // elements (= bytes) of a stage: one scale block, one swizzle row
+constexpr int F8_GROUP = 4;                      // stages served by one scale tile
+constexpr int F8_EPI_WARPS = 8;
+constexpr int F8_THREADS = 128 + 32 * F8_EPI_WARPS;  // warp 0 loads, 1 MMA, 2 scales, 3 idle; then the epilogue warps
+constexpr int F8_CTRL_BYTES = 256;
+// block-scaled instruction descriptor: A = B = E4M3 (code 0), both K-major, scale type UE8M0 (bit 23), N>>3 at 17,
+// M>>4 at 24; bits 4-5 / 29-30 name the byte of W's / A's scale word
+constexpr uint32_t f8_idesc(int M, int N) { return (1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+__device__ __forceinline__ uint32_t f8_scale_byte(uint32_t b) { return (b << 4) | (b << 29); }
+
+__device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                         uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+__device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                              uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+
+// Plain scale matrix of an operand: byte (row >> shift) * ld + block; ld and the base are multiples of 4 and every
+// row can be read up to the next multiple of 4 blocks.
+struct F8Scales {
+  const unsigned char* p;
+  int64_t ld;
+  int64_t rows;  // operand rows
+  int shift;     // 0: a scale per row, 7: per 128 rows
+};
+// this lane's 16 bytes of the tile of rows r0 .. r0 + 127, blocks 4 g .. 4 g + 3
+__device__ __forceinline__ uint4 f8_scale_words(const F8Scales& s, int r0, int g, int lane) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = (int64_t)r0 + lane + 32 * i;
+    w[i] = r < s.rows ? __ldg(reinterpret_cast<const uint32_t*>(s.p + (r >> s.shift) * s.ld + 4 * g)) : 0x7f7f7f7fu;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct F8Args {
+  F8Scales sa, sw;
+  int M, N, K;
+  int tiles_m, tiles_n;
+  EpiParams ep;
+};
+
+// ---- one CTA per 128 x 128 tile ---------------------------------------------------------------------------------
+constexpr int S8_BM = 128, S8_BN = 128;
+constexpr int S8_A_BYTES = S8_BM * 128, S8_B_BYTES = S8_BN * 128;
+constexpr int S8_STAGE_BYTES = S8_A_BYTES + S8_B_BYTES;  // 32 KiB
+constexpr int S8_STAGES = 5;
+constexpr int S8_EPI_BYTES = F8_EPI_WARPS * EPI_BOX_BYTES;
+constexpr int S8_SF_BYTES = 2 * 2 * 512;                 // two buffers of (A tile, W tile)
+constexpr int S8_SMEM_BYTES = S8_STAGES * S8_STAGE_BYTES + S8_EPI_BYTES + S8_SF_BYTES + F8_CTRL_BYTES;
+constexpr int S8_SF_COL0 = 2 * S8_BN;
+static_assert(S8_SMEM_BYTES <= 232448, "shared memory budget");
+static_assert(16 * S8_STAGES + 40 + 8 * F8_EPI_WARPS + 32 <= F8_CTRL_BYTES, "control block too small");
+
+__global__ void __launch_bounds__(F8_THREADS, 1)
+gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes, const F8Args args) {
+  constexpr int STAGES = S8_STAGES;
+  constexpr uint32_t IDESC = f8_idesc(S8_BM, S8_BN);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t tiles_base = smem_u32(smem_raw);
+  const uint32_t epi_base = tiles_base + STAGES * S8_STAGE_BYTES;
+  unsigned char* epi_gen = smem_raw + STAGES * S8_STAGE_BYTES;
+  const uint32_t sf_base = epi_base + S8_EPI_BYTES;
+  unsigned char* sf_gen = epi_gen + S8_EPI_BYTES;
+  const uint32_t ctrl = sf_base + S8_SF_BYTES;
+  unsigned char* ctrl_gen = sf_gen + S8_SF_BYTES;
+  // control: full[STAGES] | empty[STAGES] | tfull[2] | tempty[2] | tmem ptr | abort | res[EPI_WARPS] | sf[2] | sfempty[2]
+  const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * STAGES;
+  const uint32_t bar_tfull = ctrl + 16 * STAGES, bar_tempty = bar_tfull + 16;
+  const uint32_t bar_res = ctrl + 16 * STAGES + 40;
+  const uint32_t bar_sf = bar_res + 8 * F8_EPI_WARPS, bar_sfempty = bar_sf + 16;
+  volatile uint32_t* tmem_ptr_slot = reinterpret_cast<volatile uint32_t*>(ctrl_gen + 16 * STAGES + 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl_gen + 16 * STAGES + 36);
+
+  if ((tiles_base & 1023u) != 0u) {
+    if (threadIdx.x == 0) atomicExch(&g_fp8_status, 9);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_tiles = args.tiles_m * args.tiles_n;
+  const int kblocks = (args.K + F8_BK - 1) / F8_BK;
+  const int kgroups = (kblocks + F8_GROUP - 1) / F8_GROUP;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar_tfull + 8 * a, 1);
+      mbar_init(bar_tempty + 8 * a, F8_EPI_WARPS);
+      mbar_init(bar_sf + 8 * a, 1);
+      mbar_init(bar_sfempty + 8 * a, 1);
+    }
+    for (int w = 0; w < F8_EPI_WARPS; ++w) mbar_init(bar_res + 8 * w, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmOut) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmRes) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ctrl + 16 * STAGES + 32), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_slot;
+
+  if (warp == 0) {
+    // ------------------------------- loads --------------------------------------------
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        const int mt = tile / args.tiles_n, nt = tile % args.tiles_n;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1, &g_fp8_status)) { ok = false; break; }
+          const uint32_t sa = tiles_base + stage * S8_STAGE_BYTES;
+          const uint32_t fb = bar_full + 8 * stage;
+          mbar_expect_tx(fb, S8_STAGE_BYTES);
+          tma_load_2d(sa, &tmA, fb, kb * F8_BK, mt * S8_BM);
+          tma_load_2d(sa + S8_A_BYTES, &tmB, fb, kb * F8_BK, nt * S8_BN);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {  // give copies in flight time to land before shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer ---------------------------------------
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, acc_phase = 0u, grp = 0;
+      bool ok = true;
+      int it = 0;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+        const int a = it & 1;
+        if (!mbar_wait(bar_tempty + 8 * a, ((acc_phase >> a) & 1u) ^ 1u, abort_flag, 2, &g_fp8_status)) { ok = false; break; }
+        acc_phase ^= 1u << a;
+        tcgen05_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(a * S8_BN);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const uint32_t buf = grp & 1u;
+          if ((kb & (F8_GROUP - 1)) == 0 &&
+              !mbar_wait(bar_sf + 8 * buf, (grp >> 1) & 1u, abort_flag, 6, &g_fp8_status)) { ok = false; break; }
+          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, 3, &g_fp8_status)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t sa = tiles_base + stage * S8_STAGE_BYTES;
+          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + S8_A_BYTES);
+          const uint32_t sfa_t = tmem_base + (uint32_t)S8_SF_COL0 + 8 * buf, sfb_t = sfa_t + 4;
+          const uint32_t idesc = IDESC | f8_scale_byte((uint32_t)(kb & (F8_GROUP - 1)));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 32 elements = 32 bytes inside the 128-byte swizzle row
+            umma_fp8(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, sfa_t, sfb_t, (kb | k) != 0 ? 1u : 0u);
+          umma_commit(bar_empty + 8 * stage);
+          if ((kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks) {
+            umma_commit(bar_sfempty + 8 * buf);
+            ++grp;
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) umma_commit(bar_tfull + 8 * a);
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------- scale tiles --------------------------------------
+    uint32_t grp = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int m0 = (tile / args.tiles_n) * S8_BM, n0 = (tile % args.tiles_n) * S8_BN;
+      uint4 wa = f8_scale_words(args.sa, m0, 0, lane), wb = f8_scale_words(args.sw, n0, 0, lane);
+      for (int g = 0; g < kgroups; ++g, ++grp) {
+        const uint32_t buf = grp & 1u, ph = (grp >> 1) & 1u;
+        const uint4 ca = wa, cb = wb;
+        if (g + 1 < kgroups) {  // the next tile's words are in flight during this one's wait
+          wa = f8_scale_words(args.sa, m0, g + 1, lane);
+          wb = f8_scale_words(args.sw, n0, g + 1, lane);
+        }
+        // the MMAs that used this buffer are done, and so is the copy that read the shared tile
+        if (!mbar_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7, &g_fp8_status)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        unsigned char* t = sf_gen + buf * 1024 + lane * 16;
+        *reinterpret_cast<uint4*>(t) = ca;
+        *reinterpret_cast<uint4*>(t + 512) = cb;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tcgen05_fence_after();
+          const uint32_t sfa_t = tmem_base + (uint32_t)S8_SF_COL0 + 8 * buf;
+          tmem_cp_sf(sfa_t, make_sf_desc(sf_base + buf * 1024));
+          tmem_cp_sf(sfa_t + 4, make_sf_desc(sf_base + buf * 1024 + 512));
+          umma_commit(bar_sf + 8 * buf);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------- epilogue warps -----------------------------------
+    const int ew = warp - 4;
+    const int quad = warp & 3;
+    const int half = ew >> 2;
+    constexpr int HALF = S8_BN / 2, NCHUNK = HALF / 16;
+    static_assert(HALF == EPI_BOX_COLS, "one staging box per epilogue warp");
+    const EpiParams& ep = args.ep;
+    const int64_t N = args.N;
+    const bool has_res = ep.residual != nullptr;
+    EpiBox eb;
+    eb.box_s = epi_base + (uint32_t)(ew * EPI_BOX_BYTES);
+    eb.row_g = epi_gen + ew * EPI_BOX_BYTES + lane * 128;
+    eb.res_bar = bar_res + 8 * ew;
+    eb.res_phase = 0u;
+    eb.swz = (uint32_t)(lane & 7);
+    uint32_t full_phase = 0u;
+    int it = 0;
+    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
+      const int a = it & 1;
+      const int m_box = (tile / args.tiles_n) * S8_BM + quad * 32;
+      const int64_t nbase = (int64_t)(tile % args.tiles_n) * S8_BN + half * HALF;
+      const int64_t m = (int64_t)m_box + lane;
+      const bool row_ok = m < args.M;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(a * S8_BN + half * HALF);
+      const EpiRow row = epi_row_setup(ep, m, row_ok, nbase, N);
+      const bool box_rows_in = m_box < args.M;
+      const bool use_res = has_res && box_rows_in;
+      epi_box_begin<1>(eb, row, use_res, lane, m_box, &tmRes);
+      EpiStep st[2];
+      epi_fetch(row, st[0], 0);
+      if (!mbar_wait(bar_tfull + 8 * a, (full_phase >> a) & 1u, abort_flag, 4, &g_fp8_status)) break;
+      full_phase ^= 1u << a;
+      tcgen05_fence_after();
+      if (!epi_box_drain<NCHUNK, false>(eb, row, ep, taddr, st, use_res, box_rows_in, lane, m_box, &tmOut, 1.f, abort_flag,
+                                        &g_fp8_status))
+        break;
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---- CTA pairs on 256 x 256 tiles -------------------------------------------------------------------------------
+// Each CTA of a cluster of two loads its own 128 rows of A and half of the W tile; the leader issues the MMAs
+// (cta_group::2, M = 256).  Tensor memory holds one 256-column accumulator and the scale tiles, so the epilogue warps
+// copy the accumulator into registers, hand it back and finish under the next tile's MMAs (as in the NVFP4 kernel).
+// Both CTAs build the scale tiles of their own A rows and of the whole W tile in their own shared memory; the leader
+// is told when both are there (bar_sfready counts two arrivals) and issues the copies for both.
+constexpr int P8_BM = 128, P8_BN = 256;
+constexpr int P8_A_BYTES = P8_BM * 128, P8_B_BYTES = (P8_BN / 2) * 128;
+constexpr int P8_STAGE_BYTES = P8_A_BYTES + P8_B_BYTES;  // 32 KiB
+constexpr int P8_STAGES = 5;
+constexpr int P8_NBOX = (P8_BN / 2) / EPI_BOX_COLS;
+constexpr int P8_EPI_BYTES = F8_EPI_WARPS * P8_NBOX * EPI_BOX_BYTES;
+constexpr int P8_SF_TILE = 3 * 512;                      // A rows, W rows 0..127, W rows 128..255
+constexpr int P8_SF_BYTES = P8_SF_TILE;                   // one: a copy takes far less than the four stages it serves
+constexpr int P8_SMEM_BYTES = P8_STAGES * P8_STAGE_BYTES + P8_EPI_BYTES + P8_SF_BYTES + F8_CTRL_BYTES;
+constexpr int P8_SF_COL0 = P8_BN, P8_SF_COLS = 12;
+static_assert(P8_SMEM_BYTES <= 232448, "shared memory budget");
+static_assert(16 * P8_STAGES + 40 + 8 * F8_EPI_WARPS + 48 <= F8_CTRL_BYTES, "control block too small");
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes, const F8Args args) {
+  constexpr int STAGES = P8_STAGES;
+  constexpr uint32_t IDESC = f8_idesc(256, P8_BN);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t tiles_base = smem_u32(smem_raw);
+  const uint32_t epi_base = tiles_base + STAGES * P8_STAGE_BYTES;
+  unsigned char* epi_gen = smem_raw + STAGES * P8_STAGE_BYTES;
+  const uint32_t sf_base = epi_base + P8_EPI_BYTES;
+  unsigned char* sf_gen = epi_gen + P8_EPI_BYTES;
+  const uint32_t ctrl = sf_base + P8_SF_BYTES;
+  unsigned char* ctrl_gen = sf_gen + P8_SF_BYTES;
+  // control: full[STAGES] | empty[STAGES] | tfull | pad | tempty | pad | tmem ptr | abort | res[EPI_WARPS] | sf[2] |
+  // sfempty[2] | sfready[2]
+  const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * STAGES;
+  const uint32_t bar_tfull = ctrl + 16 * STAGES, bar_tempty = bar_tfull + 16;
+  const uint32_t bar_res = ctrl + 16 * STAGES + 40;
+  const uint32_t bar_sf = bar_res + 8 * F8_EPI_WARPS, bar_sfempty = bar_sf + 16, bar_sfready = bar_sf + 32;
+  volatile uint32_t* tmem_ptr_slot = reinterpret_cast<volatile uint32_t*>(ctrl_gen + 16 * STAGES + 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl_gen + 16 * STAGES + 36);
+
+  if ((tiles_base & 1023u) != 0u) {  // cluster-uniform: the dynamic window starts at the same offset in every CTA
+    if (threadIdx.x == 0) atomicExch(&g_fp8_status, 9);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
+  const int num_tiles = args.tiles_m * args.tiles_n;
+  const int kblocks = (args.K + F8_BK - 1) / F8_BK;
+  const int kgroups = (kblocks + F8_GROUP - 1) / F8_GROUP;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_tfull, 1);
+    mbar_init(bar_tempty, 2 * F8_EPI_WARPS);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar_sf + 8 * a, 1);
+      mbar_init(bar_sfempty + 8 * a, 1);
+      mbar_init(bar_sfready + 8 * a, 2);
+    }
+    for (int w = 0; w < F8_EPI_WARPS; ++w) mbar_init(bar_res + 8 * w, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmOut) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmRes) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ctrl + 16 * STAGES + 32), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anything signals them
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_slot;
+  // 384 threads start with 168 registers each; the epilogue warps, which hold a 128-column slice of the accumulator,
+  // take over what warpgroup 0 gives up: 128 x 40 + 256 x 232 = 64 512 = 384 x 168
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  if (warp == 0) {
+    // ------------------------------- loads (both CTAs) ----------------------------------
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      const uint32_t full0 = map_to_cta(bar_full, 0);
+      for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
+        int mt, nt;
+        pair_tile_coords(tile, args.tiles_m, args.tiles_n, mt, nt);
+        const int m0 = mt * 256 + (int)rank * P8_BM;
+        const int n0 = nt * P8_BN + (int)rank * (P8_BN / 2);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1, &g_fp8_status)) { ok = false; break; }
+          const uint32_t sa = tiles_base + stage * P8_STAGE_BYTES;
+          if (leader) mbar_expect_tx(bar_full + 8 * stage, 2 * P8_STAGE_BYTES);
+          const uint32_t fb = full0 + 8 * stage;
+          tma_load_2d_pair(sa, &tmA, fb, kb * F8_BK, m0);
+          tma_load_2d_pair(sa + P8_A_BYTES, &tmB, fb, kb * F8_BK, n0);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer (leader CTA only) -----------------------
+    if (leader && lane == 0) {
+      uint32_t stage = 0, phase = 0, acc_phase = 0, grp = 0;
+      bool ok = true;
+      for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
+        if (!mbar_wait(bar_tempty, acc_phase ^ 1u, abort_flag, 2, &g_fp8_status)) { ok = false; break; }
+        acc_phase ^= 1u;
+        tcgen05_fence_after();
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const uint32_t buf = grp & 1u;
+          if ((kb & (F8_GROUP - 1)) == 0 &&
+              !mbar_wait(bar_sf + 8 * buf, (grp >> 1) & 1u, abort_flag, 6, &g_fp8_status)) { ok = false; break; }
+          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, 3, &g_fp8_status)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t sa = tiles_base + stage * P8_STAGE_BYTES;
+          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + P8_A_BYTES);
+          const uint32_t sfa_t = tmem_base + (uint32_t)P8_SF_COL0 + P8_SF_COLS * buf, sfb_t = sfa_t + 4;
+          const uint32_t idesc = IDESC | f8_scale_byte((uint32_t)(kb & (F8_GROUP - 1)));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_fp8_pair(tmem_base, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, sfa_t, sfb_t,
+                          (kb | k) != 0 ? 1u : 0u);
+          umma_commit_pair(bar_empty + 8 * stage);  // frees this stage in both CTAs
+          if ((kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks) {
+            tc_commit_pair_local(bar_sfempty + 8 * buf);
+            ++grp;
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) umma_commit_pair(bar_tfull);  // accumulator complete, both CTAs
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------- scale tiles (both CTAs build, the leader copies) ----
+    uint32_t grp = 0;
+    bool ok = true;
+    const uint32_t ready0 = map_to_cta(bar_sfready, 0);
+    for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
+      int mt, nt;
+      pair_tile_coords(tile, args.tiles_m, args.tiles_n, mt, nt);
+      const int m0 = mt * 256 + (int)rank * P8_BM, n0 = nt * P8_BN;
+      uint4 wa = f8_scale_words(args.sa, m0, 0, lane), wb = f8_scale_words(args.sw, n0, 0, lane),
+            wc = f8_scale_words(args.sw, n0 + 128, 0, lane);
+      for (int g = 0; g < kgroups; ++g, ++grp) {
+        const uint32_t buf = grp & 1u, ph = (grp >> 1) & 1u;
+        // the copies that read the shared tiles of the group before are done (one commit tells both CTAs)
+        if (grp > 0 && !mbar_wait(bar_sf + 8 * (buf ^ 1u), ((grp - 1) >> 1) & 1u, abort_flag, 8, &g_fp8_status)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        unsigned char* t = sf_gen + lane * 16;
+        *reinterpret_cast<uint4*>(t) = wa;
+        *reinterpret_cast<uint4*>(t + 512) = wb;
+        *reinterpret_cast<uint4*>(t + 1024) = wc;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (g + 1 < kgroups) {  // in flight while the leader waits and copies
+          wa = f8_scale_words(args.sa, m0, g + 1, lane);
+          wb = f8_scale_words(args.sw, n0, g + 1, lane);
+          wc = f8_scale_words(args.sw, n0 + 128, g + 1, lane);
+        }
+        if (lane == 0) {
+          mbar_arrive_cluster(ready0 + 8 * buf);
+          if (leader) {
+            if (!mbar_wait(bar_sfready + 8 * buf, ph, abort_flag, 9, &g_fp8_status)) ok = false;
+            // the MMAs that used this buffer's columns are done
+            if (ok && !mbar_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7, &g_fp8_status)) ok = false;
+            if (ok) {
+              tcgen05_fence_after();
+              const uint32_t sfa_t = tmem_base + (uint32_t)P8_SF_COL0 + P8_SF_COLS * buf;
+              tmem_cp_sf_pair(sfa_t, make_sf_desc(sf_base));
+              tmem_cp_sf_pair(sfa_t + 4, make_sf_desc(sf_base + 512));
+              tmem_cp_sf_pair(sfa_t + 8, make_sf_desc(sf_base + 1024));
+              umma_commit_pair(bar_sf + 8 * buf);
+            }
+          }
+        }
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      }
+    }
+  }
+  } else {
+    // ------------------------------- epilogue warps (both CTAs) -------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int ew = warp - 4;
+    const int quad = warp & 3;
+    const int half = ew >> 2;
+    constexpr int HALF = P8_BN / 2, NCHUNK = HALF / 16;
+    const EpiParams& ep = args.ep;
+    const int64_t N = args.N;
+    const bool has_res = ep.residual != nullptr;
+    const uint32_t tempty0 = map_to_cta(bar_tempty, 0);
+    EpiBox eb;
+    eb.box_s = epi_base + (uint32_t)(ew * P8_NBOX * EPI_BOX_BYTES);
+    eb.row_g = epi_gen + ew * P8_NBOX * EPI_BOX_BYTES + lane * 128;
+    eb.res_bar = bar_res + 8 * ew;
+    eb.res_phase = 0u;
+    eb.swz = (uint32_t)(lane & 7);
+    uint32_t full_phase = 0u;
+    for (int tile = cluster_id; tile < num_tiles; tile += num_clusters) {
+      int mt, nt;
+      pair_tile_coords(tile, args.tiles_m, args.tiles_n, mt, nt);
+      const int m_box = mt * 256 + (int)rank * P8_BM + quad * 32;
+      const int64_t nbase = (int64_t)nt * P8_BN + half * HALF;
+      const int64_t m = (int64_t)m_box + lane;
+      const bool row_ok = m < args.M;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * HALF);
+      const EpiRow row = epi_row_setup(ep, m, row_ok, nbase, N);
+      const bool box_rows_in = m_box < args.M;
+      const bool use_res = has_res && box_rows_in;
+      epi_box_begin<P8_NBOX>(eb, row, use_res, lane, m_box, &tmRes);
+      if (!mbar_wait(bar_tfull, full_phase, abort_flag, 4, &g_fp8_status)) break;
+      full_phase ^= 1u;
+      tcgen05_fence_after();
+      uint32_t acc[NCHUNK][16];
+      epi_acc_load<NCHUNK>(taddr, acc);
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty0);
+      if (!epi_box_drain_regs<NCHUNK, false>(eb, row, ep, acc, use_res, box_rows_in, lane, m_box, &tmOut, 1.f, abort_flag,
+                                             &g_fp8_status))
+        break;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // nobody leaves while the other CTA may still signal or read it
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---- quantiser --------------------------------------------------------------------------------------------------
+// The least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), from the bits of amax: exponent - 8, one more when the
+// fraction is above 1.75; at least -126 (which a block of zeros takes).  Returns the E8M0 byte e + 127.
+__device__ __forceinline__ uint32_t f8_scale_of(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)(max(e, -126) + 127);
+}
+// 2^-e for the byte e + 127, which lies in [1, 247] (the largest fp32 value takes e = 120)
+__device__ __forceinline__ float f8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float f8_finite_abs(float x) {  // |x|, or 0 for an infinity or NaN
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+// two values -> two E4M3 codes; a non-finite value becomes NaN (the conversion alone would saturate an infinity)
+__device__ __forceinline__ uint32_t f8_codes2(float lo, float hi, float inv) {
+  const float nan = __uint_as_float(0x7fffffffu);
+  lo = fabsf(lo) <= 3.402823466e38f ? lo * inv : nan;
+  hi = fabsf(hi) <= 3.402823466e38f ? hi * inv : nan;
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+template <typename T>
+__device__ __forceinline__ void f8_load8(const T* p, float (&f)[8]);
+template <>
+__device__ __forceinline__ void f8_load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&f)[8]) { unpack8(ldg_nc_u4(p), f); }
+template <>
+__device__ __forceinline__ void f8_load8<float>(const float* p, float (&f)[8]) {
+  const uint4 a = ldg_nc_u4(p), b = ldg_nc_u4(p + 4);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
+}
+
+// One scale for each row and 128 elements: 16 lanes hold a block, 8 elements each.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const T* __restrict__ x, int64_t ld, unsigned char* __restrict__ q,
+                                                                unsigned char* __restrict__ sf, int64_t ldsf, int64_t rows, int K,
+                                                                int kblocks) {
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;  // (row, block)
+  const int sub = threadIdx.x & 15;
+  if (unit >= rows * kblocks) return;  // 16 lanes leave together
+  const int64_t r = unit / kblocks;
+  const int kb = (int)(unit - r * kblocks);
+  const int k = kb * 128 + 8 * sub;
+  const bool in = k < K;  // K is a multiple of 16
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (in) f8_load8(x + r * ld + k, f);
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[e]));
+  const uint32_t half = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
+  const uint32_t byte = f8_scale_of(m);
+  if (sub == 0) sf[r * ldsf + kb] = (unsigned char)byte;
+  if (in) {
+    const float inv = f8_inverse(byte);
+    *reinterpret_cast<uint2*>(q + r * K + k) = make_uint2(f8_codes2(f[0], f[1], inv) | (f8_codes2(f[2], f[3], inv) << 16),
+                                                          f8_codes2(f[4], f[5], inv) | (f8_codes2(f[6], f[7], inv) << 16));
+  }
+}
+
+// One scale for each 128 x 128 block (weights, quantised once): a CTA per block, rows in 8 passes of 16.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_quantize_tiles_kernel(const T* __restrict__ x, int64_t ld, unsigned char* __restrict__ q,
+                                                                 unsigned char* __restrict__ sf, int64_t ldsf, int64_t rows, int K) {
+  __shared__ float red[8];
+  const int sub = threadIdx.x & 15, slot = threadIdx.x >> 4;
+  const int k = blockIdx.x * 128 + 8 * sub;
+  const int64_t r0 = (int64_t)blockIdx.y * 128;
+  float f[8][8];
+  float m = 0.f;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int64_t r = r0 + 16 * p + slot;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[p][e] = 0.f;
+    if (k < K && r < rows) f8_load8(x + r * ld + k, f[p]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[p][e]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+  const uint32_t byte = f8_scale_of(m);
+  if (threadIdx.x == 0) sf[blockIdx.y * ldsf + blockIdx.x] = (unsigned char)byte;
+  const float inv = f8_inverse(byte);
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int64_t r = r0 + 16 * p + slot;
+    if (k < K && r < rows)
+      *reinterpret_cast<uint2*>(q + r * K + k) =
+          make_uint2(f8_codes2(f[p][0], f[p][1], inv) | (f8_codes2(f[p][2], f[p][3], inv) << 16),
+                     f8_codes2(f[p][4], f[p][5], inv) | (f8_codes2(f[p][6], f[p][7], inv) << 16));
+  }
+}
+
+template <typename T>
+static int launch_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t ldsf, int64_t rows, int64_t K, int block_rows,
+                           cudaStream_t st) {
+  const int64_t kblocks = ceil_div(K, 128);
+  const T* xp = static_cast<const T*>(x);
+  unsigned char *qp = static_cast<unsigned char*>(q), *sp = static_cast<unsigned char*>(sf);
+  if (block_rows == 1) {
+    const int64_t blocks = ceil_div(rows * kblocks, 16);
+    SANA_REQUIRE(blocks < ((int64_t)1 << 31), "sana_fp8_quantize: too large");
+    fp8_quantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows, (int)K, (int)kblocks);
+  } else {
+    const int64_t rb = ceil_div(rows, 128);
+    SANA_REQUIRE(rb <= 65535, "sana_fp8_quantize: more than 65535 blocks of 128 rows");
+    fp8_quantize_tiles_kernel<T><<<dim3((unsigned)kblocks, (unsigned)rb), 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows, (int)K);
+  }
+  SANA_LAUNCH_CHECK("fp8_quantize kernel");
+  return SANA_OK;
+}
+
+}  // namespace sana
+
+using namespace sana;
+
+extern "C" int sana_fp8_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t ldsf, int64_t rows, int64_t K,
+                                 int block_rows, int dtype, void* stream) {
+  SANA_REQUIRE(x && q && sf, "sana_fp8_quantize: null pointer");
+  SANA_REQUIRE(rows > 0 && K > 0 && K % 16 == 0 && K < ((int64_t)1 << 30), "sana_fp8_quantize: K must be a positive multiple of 16");
+  SANA_REQUIRE(block_rows == 1 || block_rows == 128, "sana_fp8_quantize: block_rows must be 1 or 128");
+  SANA_REQUIRE(dtype == SANA_BF16 || dtype == SANA_F32, "sana_fp8_quantize: unknown dtype %d", dtype);
+  SANA_REQUIRE(ld >= K && ld % (dtype == SANA_BF16 ? 8 : 4) == 0, "sana_fp8_quantize: ld must be >= K and keep rows 16-byte aligned");
+  SANA_REQUIRE(ldsf >= ceil_div(K, 128), "sana_fp8_quantize: ldsf too small");
+  SANA_REQUIRE(rows < ((int64_t)1 << 31), "sana_fp8_quantize: too many rows");
+  SANA_REQUIRE(aligned16(x) && aligned16(q), "sana_fp8_quantize: alignment");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SANA_BF16 ? launch_quantize<__nv_bfloat16>(x, ld, q, sf, ldsf, rows, K, block_rows, st)
+                            : launch_quantize<float>(x, ld, q, sf, ldsf, rows, K, block_rows, st);
+}
+
+extern "C" int sana_gemm_fp8(const void* Aq, const void* sfa, int64_t ldsfa, int a_block_rows, const void* Wq, const void* sfw,
+                             int64_t ldsfw, int w_block_rows, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                             const sana_gemm_epilogue* ep, void* stream) {
+  SANA_REQUIRE(Aq && sfa && Wq && sfw && out, "sana_gemm_fp8: null pointer");
+  SANA_REQUIRE(M > 0 && N > 0 && K > 0, "sana_gemm_fp8: M, N, K must be positive");
+  SANA_REQUIRE(K % 16 == 0 && N % 8 == 0 && ldo >= N && ldo % 8 == 0, "sana_gemm_fp8: K %% 16, N %% 8, ldo %% 8 required");
+  SANA_REQUIRE(M < ((int64_t)1 << 31) - 256 && N < ((int64_t)1 << 31) - 256 && K < ((int64_t)1 << 30), "sana_gemm_fp8: size out of range");
+  SANA_REQUIRE((a_block_rows == 1 || a_block_rows == 128) && (w_block_rows == 1 || w_block_rows == 128),
+               "sana_gemm_fp8: block_rows must be 1 or 128");
+  const int64_t words = ceil_div(ceil_div(K, 128), 4) * 4;
+  SANA_REQUIRE(ldsfa >= words && ldsfw >= words && ldsfa % 4 == 0 && ldsfw % 4 == 0 &&
+                   (reinterpret_cast<uintptr_t>(sfa) & 3) == 0 && (reinterpret_cast<uintptr_t>(sfw) & 3) == 0,
+               "sana_gemm_fp8: scale rows must be 4-byte aligned and padded to a multiple of 4 blocks");
+  SANA_REQUIRE(aligned16(Aq) && aligned16(Wq) && aligned16(out), "sana_gemm_fp8: alignment");
+  EpiParams p;
+  int rc = check_epilogue(ep, N, &p, "sana_gemm_fp8");
+  if (rc) return rc;
+  SANA_REQUIRE(!p.residual || (aligned16(p.residual) && p.ldr % 8 == 0), "sana_gemm_fp8: residual alignment");
+  SANA_REQUIRE(!p.bias || aligned16(p.bias), "sana_gemm_fp8: bias alignment");
+  SANA_REQUIRE(!p.gate_table || (aligned16(p.gate_table) && aligned16(p.gate_t)), "sana_gemm_fp8: gate alignment");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  F8Args a;
+  a.sa = {static_cast<const unsigned char*>(sfa), ldsfa, M, a_block_rows == 128 ? 7 : 0};
+  a.sw = {static_cast<const unsigned char*>(sfw), ldsfw, N, w_block_rows == 128 ? 7 : 0};
+  a.M = (int)M, a.N = (int)N, a.K = (int)K;
+  a.ep = p;
+  CUtensorMap tmA, tmB, tmOut, tmRes;
+  rc = make_tmap_2d(&tmOut, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, M, N, ldo * 2, 32, EPI_BOX_COLS);
+  if (rc) return rc;
+  tmRes = tmOut;
+  if (p.residual) {
+    rc = make_tmap_2d(&tmRes, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.residual, M, N, p.ldr * 2, 32, EPI_BOX_COLS);
+    if (rc) return rc;
+  }
+  const int variant = gemm_variant();
+  const bool pair = variant == 2 || (variant == 0 && M >= 2048);
+  rc = make_tmap_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, Aq, M, K, K, 128, F8_BK);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, Wq, N, K, K, 128, F8_BK);
+  if (rc) return rc;
+  if (pair) {
+    static OncePerDevice once;
+    if (once.first_time()) {
+      cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM_BYTES);
+      if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_fp8_pair)");
+    }
+    a.tiles_m = (int)ceil_div(M, 256);
+    a.tiles_n = (int)ceil_div(N, P8_BN);
+    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+    SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
+    const int64_t max_clusters = sm_count() / 2;
+    const int grid = (int)(2 * (tiles < max_clusters ? tiles : max_clusters));
+    gemm_fp8_pair_kernel<<<grid, F8_THREADS, P8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
+    SANA_LAUNCH_CHECK("gemm_fp8_pair kernel");
+    return SANA_OK;
+  }
+  static OncePerDevice once;
+  if (once.first_time()) {
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S8_SMEM_BYTES);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_fp8_tc)");
+  }
+  a.tiles_m = (int)ceil_div(M, S8_BM);
+  a.tiles_n = (int)ceil_div(N, S8_BN);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
+  const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
+  gemm_fp8_tc_kernel<<<grid, F8_THREADS, S8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
+  SANA_LAUNCH_CHECK("gemm_fp8_tc kernel");
+  return SANA_OK;
+}
+
+extern "C" int sana_gemm_fp8_take_device_status(int* status_out) {
+  if (!status_out) return fail(SANA_ERR_INVALID, "sana_gemm_fp8_take_device_status: null pointer");
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_fp8_status, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "cudaMemcpyFromSymbol(g_fp8_status)");
+  if (v != 0) {
+    int zero = 0;
+    e = cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return cuda_status(e, "cudaMemcpyToSymbol(g_fp8_status)");
+  }
+  *status_out = v;
+  return SANA_OK;
+}

@@ -463,6 +463,25 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
                : "memory");
 }
 
+// ---- scale tiles of the block-scaled kernels: shared memory -> tensor memory ----------------------
+// 32 rows x 16 bytes, rows contiguous: 8-row groups 128 bytes apart, no swizzle
+__device__ __forceinline__ uint64_t make_sf_desc(uint32_t saddr) {
+  const uint32_t lo = (saddr >> 4) & 0x3FFFu;
+  const uint32_t hi = (128u >> 4) | (1u << 14);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+__device__ __forceinline__ void tmem_cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// arrive (once, on this CTA's barrier) when every tcgen05 operation this thread has issued so far is complete
+__device__ __forceinline__ void tc_commit_pair_local(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // Order of the output tiles.  Row-major order makes the tiles in flight at one time (one per CTA pair) span two
 // tile rows and every tile column, i.e. the whole weight matrix passes through L2 once per wave (50 MB for the
 // 11 200-wide projection).  Walking groups of PAIR_GROUP_M tile rows column by column keeps a wave on a few

@@ -717,3 +717,109 @@ def take_gemm_nvfp4_device_status() -> int:
     lib = _lib.load()
     _lib.check(lib.sana_gemm_nvfp4_take_device_status(C.byref(v)), "sana_gemm_nvfp4_take_device_status")
     return v.value
+
+
+FP8_BLOCK = 128  # elements along K that share a scale
+
+
+def _device_of(what: str, *ts: Optional[torch.Tensor]) -> int:
+    """Index of the one CUDA device that all given tensors live on."""
+    index = -1
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise SanaLibraryError("sana_b200 operators run on CUDA tensors only (no CPU path)")
+        if index < 0:
+            index = t.device.index
+        elif t.device.index != index:
+            raise SanaLibraryError(f"{what}: tensors on different devices")
+    return index
+
+
+class Fp8Tensor:
+    """A [rows, K] matrix as E4M3 codes ``q`` (float8_e4m3fn, contiguous) with one power-of-two scale for each block of
+    ``block_rows`` rows x 128 columns: ``scales`` [ceil(rows / block_rows), ceil(K / 128)] uint8 holds exponent + 127
+    (E8M0).  Scale rows are read in words of four, so ``scales`` is copied here when its rows are not padded that far."""
+
+    __slots__ = ("q", "scales", "block_rows", "rows", "K")
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, block_rows: int = 1):
+        if q.dim() != 2 or q.dtype != torch.float8_e4m3fn or not q.is_contiguous():
+            raise SanaLibraryError("Fp8Tensor: codes must be a contiguous float8_e4m3fn matrix")
+        if block_rows not in (1, FP8_BLOCK):
+            raise SanaLibraryError("Fp8Tensor: block_rows must be 1 or 128")
+        self.rows, self.K = q.shape
+        kb = (self.K + FP8_BLOCK - 1) // FP8_BLOCK
+        if scales.dtype == torch.float8_e8m0fnu:
+            scales = scales.view(torch.uint8)
+        if scales.dtype != torch.uint8 or scales.shape != ((self.rows + block_rows - 1) // block_rows, kb):
+            raise SanaLibraryError("Fp8Tensor: scales must be uint8 (or float8_e8m0fnu) "
+                                   f"[ceil(rows / {block_rows}), ceil(K / 128)]")
+        words = (kb + 3) // 4 * 4
+        ld = scales.stride(0)
+        if not (scales.stride(1) == 1 or kb == 1) or ld < words or ld % 4 or scales.data_ptr() % 4 or \
+                scales.storage_offset() + (scales.shape[0] - 1) * ld + words > scales.untyped_storage().nbytes():
+            padded = torch.zeros(scales.shape[0], words, dtype=torch.uint8, device=scales.device)
+            padded[:, :kb] = scales
+            scales = padded[:, :kb]
+        self.q, self.scales, self.block_rows = q, scales, block_rows
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [rows, K] reconstruction (torch math; for tests and diagnostics only)."""
+        e = self.scales.to(torch.int32).repeat_interleave(self.block_rows, 0)[:self.rows]
+        return torch.ldexp(self.q.float(), e.repeat_interleave(FP8_BLOCK, 1)[:, :self.K] - 127)
+
+
+def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
+    """Quantises a bf16 or fp32 [rows, K] matrix (contiguous rows, K a multiple of 16) to E4M3 with one power-of-two
+    scale for each 128 elements of a row (``block_rows=1``, activations) or each 128 x 128 block (128, weights).
+    An infinity or NaN becomes NaN and leaves its block's scale alone."""
+    dev = _device_of("fp8_quantize", x)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return fp8_quantize(x, block_rows)
+    rows, K, ld = _rows2d(x, "fp8_quantize x")
+    if K % 16 != 0 or K == 0 or rows == 0:
+        raise SanaLibraryError("fp8_quantize: K must be a positive multiple of 16, and there must be rows")
+    if block_rows not in (1, FP8_BLOCK):
+        raise SanaLibraryError("fp8_quantize: block_rows must be 1 or 128")
+    kb = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    q = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=x.device)
+    words = (kb + 3) // 4 * 4
+    sf = torch.empty((rows + block_rows - 1) // block_rows, words, dtype=torch.uint8, device=x.device)
+    _lib.check(_lib.load().sana_fp8_quantize(x.data_ptr(), ld if rows > 1 else max(ld, K), q.data_ptr(), sf.data_ptr(), words,
+                                             rows, K, block_rows, _dtype_code(x.dtype), _stream()), "sana_fp8_quantize")
+    counters.launches += 1
+    return Fp8Tensor(q, sf[:, :kb], block_rows)
+
+
+def gemm_fp8(a: Fp8Tensor, w: Fp8Tensor, bias=None, act: int = ACT_NONE, relu_cols: int = 0, gate=None,
+             residual=None, out=None) -> torch.Tensor:
+    """out [M, N] bf16 = epilogue(dequant(a) @ dequant(w).T) on the 8-bit tensor cores; arguments as :func:`gemm`.
+    N must be a multiple of 8."""
+    if a.K != w.K:
+        raise SanaLibraryError(f"gemm_fp8: K mismatch ({a.K} vs {w.K})")
+    dev = _device_of("gemm_fp8", a.q, a.scales, w.q, w.scales, bias, residual, out, *(gate[:2] if gate is not None else ()))
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return gemm_fp8(a, w, bias, act, relu_cols, gate, residual, out)
+    M, Nn, K = a.rows, w.rows, a.K
+    if out is None:
+        out = torch.empty(M, Nn, dtype=torch.bfloat16, device=a.q.device)
+    Mo, No, ldo = _rows2d(out, "gemm_fp8 out")
+    if Mo != M or No != Nn or out.dtype != torch.bfloat16:
+        raise SanaLibraryError("gemm_fp8: bad output tensor")
+    ep, keep = _epilogue(M, Nn, torch.bfloat16, bias, act, relu_cols, gate, residual)
+    _lib.check(_lib.load().sana_gemm_fp8(a.q.data_ptr(), a.scales.data_ptr(), a.scales.stride(0), a.block_rows, w.q.data_ptr(),
+                                         w.scales.data_ptr(), w.scales.stride(0), w.block_rows, out.data_ptr(), ldo, M, Nn, K,
+                                         C.byref(ep), _stream()), "sana_gemm_fp8")
+    counters.launches += 1
+    return out
+
+
+def take_gemm_fp8_device_status() -> int:
+    """Code recorded by a timed-out wait inside the 8-bit GEMM (0 = none).  Synchronises."""
+    v = C.c_int(0)
+    _lib.check(_lib.load().sana_gemm_fp8_take_device_status(C.byref(v)), "sana_gemm_fp8_take_device_status")
+    return int(v.value)
