@@ -241,6 +241,44 @@ int sana_la_rope_apply(const void* q, int64_t ldq, const float* cos_table, const
 int sana_la_rope_take_device_status(int* status_out);
 
 /* ---------------------------------------------------------------------------------------
+ * Causal linear attention with a decay for each head.  With lambda_h = exp(log_decay[h]) (log_decay <= 0; -inf forgets
+ * everything) and phi the identity, or ReLU when `relu` is set:
+ *   S_t = lambda_h S_{t-1} + [v_t ; 1] (x) phi(k_t)                       [D+1, D] per head, row D = the key sum
+ *   o_t = scale * S_t[:D] phi(q_t)                                        eps < 0
+ *   o_t = S_t[:D] phi(q_t) / (S_t[D] . phi(q_t) + eps)                    eps >= 0 (needs relu; scale unused)
+ * The token-causal, forgetting form of sana_la_state + sana_la_apply: with log_decay = 0 the state after the last token
+ * is theirs, in the layout of sana_la_rope_state.  No counterpart upstream (its causal attention, sana_blocks.py:391-572,
+ * is causal over whole chunks of frames and keeps everything).
+ *   q, out [B*N, *] rows of H*D channels (head-major), k, v [B*N, *] rows of Hk*D channels; H a
+ *   multiple of Hk (query head h reads key/value head h / (H / Hk)); D a multiple of 16 in [16, 128]; rows 16-byte aligned
+ *   log_decay [H] fp32;  prior [B, H, D+1, D] fp32 (the state before the first token) or NULL;  state: the state after
+ *   the last token, a buffer other than prior
+ *   lengths [B] int32 on the device, or NULL: sequence b has lengths[b] tokens (clamped to [0, N]); the rows behind them
+ *   are not read, their outputs are zeros, and the state is the one after token lengths[b] - 1 (or prior, or zeros)
+ *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
+ *   arguments), 16-byte aligned.
+ * State, decays and normalisers are fp32; bf16: both sides of the products are bf16, the state enters the product with q
+ * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once.  Bit-reproducible.  A NaN or
+ * infinity among the valid tokens reaches every later output of its heads, and may reach outputs up to 15 tokens
+ * before it (bf16) in the unnormalised and the normalised form alike.
+ *
+ * sana_la_decay_step: one token of each of B sequences.  q, k, v, out hold B rows; state [pool, H, D+1, D] is updated in
+ * place, row b of the batch using entry slots[b] (slots [B] int32 on the device, or NULL for entry b).  A slot of -1
+ * marks a row without a sequence: its output is zeros.  A slot outside [-1, pool), or one that an earlier row of the
+ * batch names already, leaves the state alone and gives NaN outputs.
+ */
+int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype);
+int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                  const float* log_decay,
+                  const float* prior, const int32_t* lengths, float* state, void* out, int64_t ldo, void* workspace,
+                  int64_t workspace_bytes, int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t D, float scale,
+                  int relu, float eps, int dtype, void* stream);
+int sana_la_decay_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                  const float* log_decay,
+                       float* state, int64_t pool, const int32_t* slots, void* out, int64_t ldo, int64_t B, int64_t H,
+                       int64_t Hk, int64_t D, float scale, int relu, float eps, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * 3x3 depthwise conv + bias + SiLU-GLU on channels-last rows:
  *   w[y, x, c]  = b[c] + sum_{dy,dx} K[c, dy, dx] * u[y+dy-1, x+dx-1, c]   (zero outside a frame)
  *   out[y, x, c] = w[y, x, c] * silu(w[y, x, hid + c]),  c in [0, hid)

@@ -66,6 +66,11 @@ SIGNATURES = {
     "sana_la_rope_state_add": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
     "sana_add_f32": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "sana_la_rope_apply": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
+    "sana_la_decay_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32]),
+    "sana_la_decay": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _f32, _i32, _f32, _i32, _vp]),
+    "sana_la_decay_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32,
+                                  _i32, _f32, _i32, _vp]),
     "sana_cross_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
     "sana_cross_attention_set_variant": (_i32, [_i32]),
     "sana_cross_attention_take_device_status": (_i32, [C.POINTER(C.c_int)]),

@@ -823,3 +823,104 @@ def take_gemm_fp8_device_status() -> int:
     v = C.c_int(0)
     _lib.check(_lib.load().sana_gemm_fp8_take_device_status(C.byref(v)), "sana_gemm_fp8_take_device_status")
     return int(v.value)
+
+
+def _decay_inputs(what: str, q, k, v, log_decay, rows: int, H: int, D: int, relu: bool, eps):
+    """Row strides of q, k and v, and the number of key/value heads, after checking what both forms share."""
+    rq, cq, ldq = _rows2d(q, what + " q")
+    rk, ck, ldk = _rows2d(k, what + " k")
+    rv, cv, ldv = _rows2d(v, what + " v")
+    if D < 16 or D > 128 or D % 16:
+        raise SanaLibraryError(f"{what}: head dimension {D} is not a multiple of 16 in [16, 128]")
+    if rq != rows or cq != H * D or rk != rows or rv != rows or ck != cv or ck % D or ck == 0 or H % (ck // D):
+        raise SanaLibraryError(f"{what}: q must be [{rows}, H*D] and k, v [{rows}, Hk*D] with H a multiple of Hk")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise SanaLibraryError(f"{what}: q, k, v must share a dtype")
+    if log_decay.dtype != torch.float32 or log_decay.shape != (H,) or not log_decay.is_contiguous():
+        raise SanaLibraryError(f"{what}: log_decay must be contiguous fp32 [H]")
+    if eps is not None and (not relu or not eps >= 0):
+        raise SanaLibraryError(f"{what}: the normalised form needs the ReLU features and eps >= 0")
+    if rows == 1:  # the stride of a single row is never used; a caller's may be anything
+        ldq, ldk, ldv = cq, ck, ck
+    return ldq, ldk, ldv, ck // D
+
+
+def _int32_vector(t: Optional[torch.Tensor], n: int, what: str) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise SanaLibraryError(f"{what} must be a contiguous int32 tensor [{n}]")
+    return t.data_ptr()
+
+
+def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, B: int, N: int, H: int, D: int,
+             scale: float = 1.0, relu: bool = False, eps: Optional[float] = None, prior: Optional[torch.Tensor] = None,
+             lengths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Causal linear attention with a decay for each head over whole prompts (see sana_la_decay):
+    ``S_t = exp(log_decay) S_{t-1} + [v_t; 1] phi(k_t)^T``, ``o_t = scale * S_t[:D] phi(q_t)``, or with ``eps``
+    ``S_t[:D] phi(q_t) / (S_t[D] . phi(q_t) + eps)``; phi is ReLU with ``relu``, else the identity.
+
+    q [B*N, H*D] and k, v [B*N, Hk*D] views (column blocks of a projection), H a multiple of Hk; log_decay fp32 [H], not
+    positive; prior fp32 [B, H, D+1, D], the state carried in; lengths int32 [B] for a padded batch (rows behind a
+    sequence give zeros).  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
+    dev = _device_of("la_decay", q, k, v, log_decay, prior, lengths, out)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return la_decay(q, k, v, log_decay, B, N, H, D, scale, relu, eps, prior, lengths, out)
+    if B < 1 or N < 1 or H < 1:
+        raise SanaLibraryError("la_decay: B, N and H must be positive")
+    ldq, ldk, ldv, Hk = _decay_inputs("la_decay", q, k, v, log_decay, B * N, H, D, relu, eps)
+    dt = _dtype_code(q.dtype)
+    if prior is not None and (prior.shape != (B, H, D + 1, D) or prior.dtype != torch.float32 or not prior.is_contiguous()):
+        raise SanaLibraryError("la_decay: prior must be contiguous fp32 [B, H, D+1, D]")
+    lens = _int32_vector(lengths, B, "la_decay: lengths")
+    if out is None:
+        out = torch.empty(B * N, H * D, dtype=q.dtype, device=q.device)
+    ro, co, ldo = _rows2d(out, "la_decay out")
+    if ro != B * N or co != H * D or out.dtype != q.dtype:
+        raise SanaLibraryError("la_decay: bad output tensor")
+    lib = _lib.load()
+    state = torch.empty(B, H, D + 1, D, dtype=torch.float32, device=q.device)
+    ws_bytes = lib.sana_la_decay_workspace_bytes(B, N, H, D, dt)
+    if ws_bytes < 0:
+        raise SanaLibraryError("la_decay: sizes out of range")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _lib.check(lib.sana_la_decay(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
+                                 prior.data_ptr() if prior is not None else None, lens, state.data_ptr(), out.data_ptr(), ldo,
+                                 ws.data_ptr() if ws is not None else None, ws_bytes, B, N, H, Hk, D, scale, 1 if relu else 0,
+                                 -1.0 if eps is None else eps, dt, _stream()), "sana_la_decay")
+    counters.launches += 2 if ws_bytes else 1
+    return out, state
+
+
+def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, H: int,
+                  D: int, scale: float = 1.0, relu: bool = False, eps: Optional[float] = None,
+                  slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of each of B sequences through :func:`la_decay`'s recurrence: q [B, H*D], k, v [B, Hk*D]; ``state`` fp32
+    [pool, H, D+1, D] is updated in place, row b using entry ``slots[b]`` (int32 [B]; without it, entry b).  A slot of -1
+    marks an unused row (output zeros); a slot outside the pool, or one an earlier row names already, gives NaN outputs
+    and leaves the state alone.  Returns out [B, H*D]."""
+    dev = _device_of("la_decay_step", q, k, v, log_decay, state, slots, out)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return la_decay_step(q, k, v, log_decay, state, H, D, scale, relu, eps, slots, out)
+    B = q.shape[0]
+    if B < 1 or H < 1:
+        raise SanaLibraryError("la_decay_step: there must be rows and heads")
+    ldq, ldk, ldv, Hk = _decay_inputs("la_decay_step", q, k, v, log_decay, B, H, D, relu, eps)
+    if state.dim() != 4 or state.shape[1:] != (H, D + 1, D) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise SanaLibraryError("la_decay_step: state must be contiguous fp32 [pool, H, D+1, D]")
+    if slots is None and state.shape[0] != B:
+        raise SanaLibraryError("la_decay_step: without slots the state must hold one entry per row")
+    ids = _int32_vector(slots, B, "la_decay_step: slots")
+    if out is None:
+        out = torch.empty(B, H * D, dtype=q.dtype, device=q.device)
+    ro, co, ldo = _rows2d(out, "la_decay_step out")
+    if ro != B or co != H * D or out.dtype != q.dtype:
+        raise SanaLibraryError("la_decay_step: bad output tensor")
+    _lib.check(_lib.load().sana_la_decay_step(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
+                                              state.data_ptr(), state.shape[0], ids, out.data_ptr(), ldo if B > 1 else max(ldo, co),
+                                              B, H, Hk, D, scale, 1 if relu else 0, -1.0 if eps is None else eps,
+                                              _dtype_code(q.dtype), _stream()), "sana_la_decay_step")
+    counters.launches += 1
+    return out
