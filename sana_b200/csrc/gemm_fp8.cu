@@ -571,32 +571,44 @@ __device__ __forceinline__ void f8_load8<float>(const float* p, float (&f)[8]) {
   for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
 }
 
-// One scale for each row and 128 elements: 16 lanes hold a block, 8 elements each.
-template <typename T>
+// One scale for each row and 128 elements: 16 lanes hold a block, 8 elements each, of R rows at a time (their loads are
+// in flight together; R = 1 where there are few rows, so that more CTAs share the work).
+template <typename T, int R>
 __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const T* __restrict__ x, int64_t ld, unsigned char* __restrict__ q,
                                                                 unsigned char* __restrict__ sf, int64_t ldsf, int64_t rows, int K,
                                                                 int kblocks) {
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;  // (row, block)
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;  // (group of R rows, block)
   const int sub = threadIdx.x & 15;
-  if (unit >= rows * kblocks) return;  // 16 lanes leave together
-  const int64_t r = unit / kblocks;
-  const int kb = (int)(unit - r * kblocks);
+  const uint32_t group = (uint32_t)unit / (uint32_t)kblocks;  // the host keeps the units below 2^31
+  const int64_t r0 = (int64_t)group * R;
+  if (r0 >= rows) return;  // 16 lanes leave together
+  const int kb = (int)((uint32_t)unit - group * (uint32_t)kblocks);
   const int k = kb * 128 + 8 * sub;
   const bool in = k < K;  // K is a multiple of 16
-  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (in) f8_load8(x + r * ld + k, f);
-  float m = 0.f;
+  float f[R][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[e]));
+  for (int i = 0; i < R; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+    if (in && r0 + i < rows) f8_load8(x + (r0 + i) * ld + k, f[i]);
+  }
   const uint32_t half = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
-  const uint32_t byte = f8_scale_of(m);
-  if (sub == 0) sf[r * ldsf + kb] = (unsigned char)byte;
-  if (in) {
-    const float inv = f8_inverse(byte);
-    *reinterpret_cast<uint2*>(q + r * K + k) = make_uint2(f8_codes2(f[0], f[1], inv) | (f8_codes2(f[2], f[3], inv) << 16),
-                                                          f8_codes2(f[4], f[5], inv) | (f8_codes2(f[6], f[7], inv) << 16));
+  for (int i = 0; i < R; ++i) {
+    if (r0 + i >= rows) break;  // the same for the 16 lanes
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[i][e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
+    const uint32_t byte = f8_scale_of(m);
+    if (sub == 0) sf[(r0 + i) * ldsf + kb] = (unsigned char)byte;
+    if (in) {
+      const float inv = f8_inverse(byte);
+      *reinterpret_cast<uint2*>(q + (r0 + i) * K + k) =
+          make_uint2(f8_codes2(f[i][0], f[i][1], inv) | (f8_codes2(f[i][2], f[i][3], inv) << 16),
+                     f8_codes2(f[i][4], f[i][5], inv) | (f8_codes2(f[i][6], f[i][7], inv) << 16));
+    }
   }
 }
 
@@ -645,9 +657,14 @@ static int launch_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t
   const T* xp = static_cast<const T*>(x);
   unsigned char *qp = static_cast<unsigned char*>(q), *sp = static_cast<unsigned char*>(sf);
   if (block_rows == 1) {
-    const int64_t blocks = ceil_div(rows * kblocks, 16);
-    SANA_REQUIRE(blocks < ((int64_t)1 << 31), "sana_fp8_quantize: too large");
-    fp8_quantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows, (int)K, (int)kblocks);
+    const int64_t most = (int64_t)1 << 31;
+    SANA_REQUIRE(ceil_div(rows, 4) * kblocks < most, "sana_fp8_quantize: too large");
+    if (ceil_div(rows, 4) * kblocks >= 16 * 8 * (int64_t)sm_count())  // eight CTAs per SM are left with four rows each
+      fp8_quantize_rows_kernel<T, 4><<<(unsigned)ceil_div(ceil_div(rows, 4) * kblocks, 16), 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows,
+                                                                                                         (int)K, (int)kblocks);
+    else
+      fp8_quantize_rows_kernel<T, 1><<<(unsigned)ceil_div(rows * kblocks, 16), 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows, (int)K,
+                                                                                          (int)kblocks);
   } else {
     const int64_t rb = ceil_div(rows, 128);
     SANA_REQUIRE(rb <= 65535, "sana_fp8_quantize: more than 65535 blocks of 128 rows");

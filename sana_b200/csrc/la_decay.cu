@@ -341,20 +341,12 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
                                     8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    // state update: S = lambda^nv S + (weighted v)^T k
+    // state update: S = lambda^nv S + (weighted v)^T k.  The tensor core truncates its fp32 sums, so a chunk is summed on
+    // its own, smallest terms first, and joined to the state by one rounded multiply-add.
     const float whole = pow_s[nv];
+    uint32_t va[4][3][4], wa[4][2];  // three terms of the weighted v (A operand); terms of the weights in rows 0..2
 #pragma unroll
-    for (int n = 0; n < 2 * KT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[n][e] *= whole;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) zacc[n][e] *= whole;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (16 * kt >= nv) break;
-      uint32_t va[3][4], wa[2];  // three terms of the weighted v (A operand); terms of the weights in rows 0..2
+    for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // tokens 16 kt + 8 e + c2, + 1
         const int left = nv - 1 - (16 * kt + 8 * e + c2);
@@ -363,25 +355,42 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
         for (int r = 0; r < 2; ++r) {  // channels 0-7, 8-15: fragment register vf[2 r + e], A register 2 e + r
           float x = bf16_lo(vf[kt][2 * r + e]) * w0, y = bf16_hi(vf[kt][2 * r + e]) * w1;
 #pragma unroll
-          for (int s = 0; s < 3; ++s) va[s][2 * e + r] = ld_split(x, y);
+          for (int s = 0; s < 3; ++s) va[kt][s][2 * e + r] = ld_split(x, y);
         }
-        uint32_t t0 = ld_split(w0, w1), t1 = ld_split(w0, w1), t2 = ld_split(w0, w1);
-        wa[e] = g == 0 ? t0 : g == 1 ? t1 : g == 2 ? t2 : 0u;
+        const uint32_t t0 = ld_split(w0, w1), t1 = ld_split(w0, w1), t2 = ld_split(w0, w1);
+        wa[kt][e] = g == 0 ? t0 : g == 1 ? t1 : g == 2 ? t2 : 0u;
       }
 #pragma unroll
-      for (int n = 0; n < KT; ++n) {
-        uint32_t kb[4];  // k[tokens][16 n ..] as the B operand of two column tiles
-        ldsm_x4_t(kb, Ks + kt * 16 * T::ROW + off_rows + n * 32);
-        if (relu) ld_relu4(kb);
+    for (int n = 0; n < KT; ++n) {
+      uint32_t kb[4][4];  // k[tokens][16 n ..] as the B operand of two column tiles
+      float d[2][4] = {};
 #pragma unroll
-        for (int s = 0; s < 3; ++s) {
-          mma_bf16_16816(S[2 * n], va[s][0], va[s][1], va[s][2], va[s][3], kb[0], kb[1]);
-          mma_bf16_16816(S[2 * n + 1], va[s][0], va[s][1], va[s][2], va[s][3], kb[2], kb[3]);
+      for (int kt = 0; kt < 4; ++kt) {
+        ldsm_x4_t(kb[kt], Ks + kt * 16 * T::ROW + off_rows + n * 32);
+        if (relu) ld_relu4(kb[kt]);
+      }
+#pragma unroll
+      for (int s = 2; s >= 0; --s)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          mma_bf16_16816(d[0], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][0], kb[kt][1]);
+          mma_bf16_16816(d[1], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][2], kb[kt][3]);
         }
-        if (n == wh) {
-          mma_bf16_16816(zacc[0], wa[0], 0u, wa[1], 0u, kb[0], kb[1]);
-          mma_bf16_16816(zacc[1], wa[0], 0u, wa[1], 0u, kb[2], kb[3]);
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[2 * n + r][e] = fmaf(whole, S[2 * n + r][e], d[r][e]);
+      if (n == wh) {
+        float z[2][4] = {};
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          mma_bf16_16816(z[0], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][0], kb[kt][1]);
+          mma_bf16_16816(z[1], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][2], kb[kt][3]);
         }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) zacc[r][e] = fmaf(whole, zacc[r][e], z[r][e]);
       }
     }
     if (OUT) publish_z();
