@@ -76,6 +76,108 @@ struct F8Args {
   EpiParams ep;
 };
 
+// ---- epilogue ---------------------------------------------------------------------------------------------------
+// An epilogue warp owns 32 rows x 64 columns, copied out of tensor memory into 64 registers a lane (one row each).  The
+// small per-column operands live in the lanes, lane l holding columns l and 32 + l, and are passed around by shuffles:
+// 16-byte loads per row and step, as the bf16 kernel does them, took 48 more registers, and the spills went through L2
+// (shared memory leaves no L1): 8 100 cycles a tile against 2 600 now.  ACT is a template argument because eight unrolled
+// steps with every activation's code in each of them do not fit the instruction cache.
+constexpr int F8_COLS = EPI_BOX_COLS;
+struct F8Cols {
+  float bias[2], gate[2];
+  bool per_row;  // the 32 rows belong to more than one batch element: gates are read row by row
+};
+__device__ __forceinline__ float f8_bf16(const void* p, int64_t i) { return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]); }
+
+__device__ __forceinline__ F8Cols f8_cols(const EpiParams& ep, int m_box, int M, int64_t nbase, int64_t N, int lane) {
+  F8Cols c;
+  const int64_t b0 = m_box / ep.rows_per_batch;
+  c.per_row = ep.gate_table != nullptr && (min(m_box + 31, M - 1) / ep.rows_per_batch) != b0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t n = nbase + 32 * j + lane;
+    const bool in = n < N && m_box < M;
+    c.bias[j] = ep.bias && in ? f8_bf16(ep.bias, n) : 0.f;
+    c.gate[j] = ep.gate_table && in ? f8_bf16(ep.gate_table, ep.gate_row * N + n) + f8_bf16(ep.gate_t, (b0 * 6 + ep.gate_row) * N + n) : 0.f;
+  }
+  return c;
+}
+
+template <int ACT>
+__device__ __forceinline__ bool f8_drain(EpiBox& eb, const F8Cols& cols, const EpiParams& ep, const uint32_t (&acc)[4][16], bool use_res,
+                                         bool rows_in, int lane, int m_box, int M, int64_t nbase, int64_t N, const CUtensorMap* tmOut,
+                                         volatile int* abort_flag) {
+  if (nbase >= N) return true;  // uniform
+  if (use_res) {
+    if (!mbar_wait(eb.res_bar, eb.res_phase, abort_flag, 5, &g_fp8_status)) return false;
+    eb.res_phase ^= 1u;
+  }
+  const bool has_bias = ep.bias != nullptr, has_gate = ep.gate_table != nullptr;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {  // 8 columns = 16 bytes of the row; N is a multiple of 8
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(acc[c >> 1][8 * (c & 1) + e]);
+    if (has_bias) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += __shfl_sync(0xffffffffu, cols.bias[c >> 2], (8 * c + e) & 31);
+    }
+    if (ACT == 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fast_silu(v[e]);
+    } else if (ACT == 2) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (nbase + 8 * c + e < ep.relu_cols) v[e] = v[e] < 0.f ? 0.f : v[e];
+    } else if (ACT == 3) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = gelu_tanh(v[e]);
+    }
+    if (has_gate) {
+      if (cols.per_row) {  // rare: out of line, one element at a time
+        const int64_t b = min(m_box + lane, M - 1) / ep.rows_per_batch;
+        for (int e = 0; e < 8; ++e) {
+          const int64_t n = min(nbase + 8 * c + e, N - 1);
+          const float g = f8_bf16(ep.gate_table, ep.gate_row * N + n) + f8_bf16(ep.gate_t, (b * 6 + ep.gate_row) * N + n);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = i == e ? v[i] * g : v[i];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= __shfl_sync(0xffffffffu, cols.gate[c >> 2], (8 * c + e) & 31);
+      }
+    }
+    uint4* slot = reinterpret_cast<uint4*>(eb.row_g + (((uint32_t)c ^ eb.swz) << 4));
+    if (use_res) {
+      float f[8];
+      unpack8(*slot, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += f[e];
+    }
+    *slot = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && rows_in) {
+    tma_store_2d(tmOut, eb.box_s, (int)nbase, m_box);
+    bulk_commit();
+  }
+  return true;
+}
+
+// start of a tile: once the previous tile's store has read the box, the residual is fetched into it
+__device__ __forceinline__ void f8_box_begin(const EpiBox& eb, bool use_res, int lane, int m_box, int64_t nbase, int64_t N,
+                                             const CUtensorMap* tmRes) {
+  if (lane == 0) {
+    bulk_wait_read_all();
+    if (use_res && nbase < N) {
+      mbar_expect_tx(eb.res_bar, (uint32_t)EPI_BOX_BYTES);
+      tma_load_2d(eb.box_s, tmRes, eb.res_bar, (int)nbase, m_box);
+    }
+  }
+  __syncwarp();
+}
+
 // ---- one CTA per 128 x 128 tile ---------------------------------------------------------------------------------
 constexpr int S8_BM = 128, S8_BN = 128;
 constexpr int S8_A_BYTES = S8_BM * 128, S8_B_BYTES = S8_BN * 128;
@@ -88,6 +190,7 @@ constexpr int S8_SF_COL0 = 2 * S8_BN;
 static_assert(S8_SMEM_BYTES <= 232448, "shared memory budget");
 static_assert(16 * S8_STAGES + 40 + 8 * F8_EPI_WARPS + 32 <= F8_CTRL_BYTES, "control block too small");
 
+template <int ACT>
 __global__ void __launch_bounds__(F8_THREADS, 1)
 gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes, const F8Args args) {
@@ -241,8 +344,7 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int ew = warp - 4;
     const int quad = warp & 3;
     const int half = ew >> 2;
-    constexpr int HALF = S8_BN / 2, NCHUNK = HALF / 16;
-    static_assert(HALF == EPI_BOX_COLS, "one staging box per epilogue warp");
+    static_assert(S8_BN == 2 * F8_COLS, "two warps share a row of the tile");
     const EpiParams& ep = args.ep;
     const int64_t N = args.N;
     const bool has_res = ep.residual != nullptr;
@@ -257,25 +359,20 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
       const int a = it & 1;
       const int m_box = (tile / args.tiles_n) * S8_BM + quad * 32;
-      const int64_t nbase = (int64_t)(tile % args.tiles_n) * S8_BN + half * HALF;
-      const int64_t m = (int64_t)m_box + lane;
-      const bool row_ok = m < args.M;
-      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(a * S8_BN + half * HALF);
-      const EpiRow row = epi_row_setup(ep, m, row_ok, nbase, N);
-      const bool box_rows_in = m_box < args.M;
-      const bool use_res = has_res && box_rows_in;
-      epi_box_begin<1>(eb, row, use_res, lane, m_box, &tmRes);
-      EpiStep st[2];
-      epi_fetch(row, st[0], 0);
+      const int64_t nbase = (int64_t)(tile % args.tiles_n) * S8_BN + half * F8_COLS;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(a * S8_BN + half * F8_COLS);
+      const bool rows_in = m_box < args.M, use_res = has_res && rows_in;
+      f8_box_begin(eb, use_res, lane, m_box, nbase, N, &tmRes);
+      const F8Cols cols = f8_cols(ep, m_box, args.M, nbase, N, lane);
       if (!mbar_wait(bar_tfull + 8 * a, (full_phase >> a) & 1u, abort_flag, 4, &g_fp8_status)) break;
       full_phase ^= 1u << a;
       tcgen05_fence_after();
-      if (!epi_box_drain<NCHUNK, false>(eb, row, ep, taddr, st, use_res, box_rows_in, lane, m_box, &tmOut, 1.f, abort_flag,
-                                        &g_fp8_status))
-        break;
+      uint32_t acc[4][16];
+      epi_acc_load<4>(taddr, acc);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
+      if (!f8_drain<ACT>(eb, cols, ep, acc, use_res, rows_in, lane, m_box, args.M, nbase, N, &tmOut, abort_flag)) break;
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -299,16 +396,19 @@ constexpr int P8_BM = 128, P8_BN = 256;
 constexpr int P8_A_BYTES = P8_BM * 128, P8_B_BYTES = (P8_BN / 2) * 128;
 constexpr int P8_STAGE_BYTES = P8_A_BYTES + P8_B_BYTES;  // 32 KiB
 constexpr int P8_STAGES = 5;
-constexpr int P8_NBOX = (P8_BN / 2) / EPI_BOX_COLS;
-constexpr int P8_EPI_BYTES = F8_EPI_WARPS * P8_NBOX * EPI_BOX_BYTES;
+constexpr int P8_EPI_WARPS = 16;                         // four per tensor-memory quadrant, 64 columns (one box) each
+constexpr int P8_THREADS = 128 + 32 * P8_EPI_WARPS;
+constexpr int P8_EPI_BYTES = P8_EPI_WARPS * EPI_BOX_BYTES;
+constexpr int P8_CTRL_BYTES = 512;
 constexpr int P8_SF_TILE = 3 * 512;                      // A rows, W rows 0..127, W rows 128..255
 constexpr int P8_SF_BYTES = P8_SF_TILE;                   // one: a copy takes far less than the four stages it serves
-constexpr int P8_SMEM_BYTES = P8_STAGES * P8_STAGE_BYTES + P8_EPI_BYTES + P8_SF_BYTES + F8_CTRL_BYTES;
+constexpr int P8_SMEM_BYTES = P8_STAGES * P8_STAGE_BYTES + P8_EPI_BYTES + P8_SF_BYTES + P8_CTRL_BYTES;
 constexpr int P8_SF_COL0 = P8_BN, P8_SF_COLS = 12;
 static_assert(P8_SMEM_BYTES <= 232448, "shared memory budget");
-static_assert(16 * P8_STAGES + 40 + 8 * F8_EPI_WARPS + 48 <= F8_CTRL_BYTES, "control block too small");
+static_assert(16 * P8_STAGES + 40 + 8 * P8_EPI_WARPS + 48 <= P8_CTRL_BYTES, "control block too small");
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
+template <int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P8_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes, const F8Args args) {
   constexpr int STAGES = P8_STAGES;
@@ -326,7 +426,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * STAGES;
   const uint32_t bar_tfull = ctrl + 16 * STAGES, bar_tempty = bar_tfull + 16;
   const uint32_t bar_res = ctrl + 16 * STAGES + 40;
-  const uint32_t bar_sf = bar_res + 8 * F8_EPI_WARPS, bar_sfempty = bar_sf + 16, bar_sfready = bar_sf + 32;
+  const uint32_t bar_sf = bar_res + 8 * P8_EPI_WARPS, bar_sfempty = bar_sf + 16, bar_sfready = bar_sf + 32;
   volatile uint32_t* tmem_ptr_slot = reinterpret_cast<volatile uint32_t*>(ctrl_gen + 16 * STAGES + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl_gen + 16 * STAGES + 36);
 
@@ -348,13 +448,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_tfull, 1);
-    mbar_init(bar_tempty, 2 * F8_EPI_WARPS);
+    mbar_init(bar_tempty, 2 * P8_EPI_WARPS);
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_sf + 8 * a, 1);
       mbar_init(bar_sfempty + 8 * a, 1);
       mbar_init(bar_sfready + 8 * a, 2);
     }
-    for (int w = 0; w < F8_EPI_WARPS; ++w) mbar_init(bar_res + 8 * w, 1);
+    for (int w = 0; w < P8_EPI_WARPS; ++w) mbar_init(bar_res + 8 * w, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
@@ -372,10 +472,6 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   cluster_sync_all();  // the peer's barriers are initialised before anything signals them
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_ptr_slot;
-  // 384 threads start with 168 registers each; the epilogue warps, which hold a 128-column slice of the accumulator,
-  // take over what warpgroup 0 gives up: 128 x 40 + 256 x 232 = 64 512 = 384 x 168
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     // ------------------------------- loads (both CTAs) ----------------------------------
     if (lane == 0) {
@@ -481,21 +577,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       }
     }
-  }
-  } else {
+  } else if (warp >= 4) {
     // ------------------------------- epilogue warps (both CTAs) -------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int ew = warp - 4;
     const int quad = warp & 3;
-    const int half = ew >> 2;
-    constexpr int HALF = P8_BN / 2, NCHUNK = HALF / 16;
+    const int part = ew >> 2;
+    static_assert(4 * F8_COLS == P8_BN, "four warps share a row of the tile");
     const EpiParams& ep = args.ep;
     const int64_t N = args.N;
     const bool has_res = ep.residual != nullptr;
     const uint32_t tempty0 = map_to_cta(bar_tempty, 0);
     EpiBox eb;
-    eb.box_s = epi_base + (uint32_t)(ew * P8_NBOX * EPI_BOX_BYTES);
-    eb.row_g = epi_gen + ew * P8_NBOX * EPI_BOX_BYTES + lane * 128;
+    eb.box_s = epi_base + (uint32_t)(ew * EPI_BOX_BYTES);
+    eb.row_g = epi_gen + ew * EPI_BOX_BYTES + lane * 128;
     eb.res_bar = bar_res + 8 * ew;
     eb.res_phase = 0u;
     eb.swz = (uint32_t)(lane & 7);
@@ -504,25 +598,20 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       int mt, nt;
       pair_tile_coords(tile, args.tiles_m, args.tiles_n, mt, nt);
       const int m_box = mt * 256 + (int)rank * P8_BM + quad * 32;
-      const int64_t nbase = (int64_t)nt * P8_BN + half * HALF;
-      const int64_t m = (int64_t)m_box + lane;
-      const bool row_ok = m < args.M;
-      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * HALF);
-      const EpiRow row = epi_row_setup(ep, m, row_ok, nbase, N);
-      const bool box_rows_in = m_box < args.M;
-      const bool use_res = has_res && box_rows_in;
-      epi_box_begin<P8_NBOX>(eb, row, use_res, lane, m_box, &tmRes);
+      const int64_t nbase = (int64_t)nt * P8_BN + part * F8_COLS;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * F8_COLS);
+      const bool rows_in = m_box < args.M, use_res = has_res && rows_in;
+      f8_box_begin(eb, use_res, lane, m_box, nbase, N, &tmRes);
+      const F8Cols cols = f8_cols(ep, m_box, args.M, nbase, N, lane);
       if (!mbar_wait(bar_tfull, full_phase, abort_flag, 4, &g_fp8_status)) break;
       full_phase ^= 1u;
       tcgen05_fence_after();
-      uint32_t acc[NCHUNK][16];
-      epi_acc_load<NCHUNK>(taddr, acc);
+      uint32_t acc[4][16];
+      epi_acc_load<4>(taddr, acc);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0);
-      if (!epi_box_drain_regs<NCHUNK, false>(eb, row, ep, acc, use_res, box_rows_in, lane, m_box, &tmOut, 1.f, abort_flag,
-                                             &g_fp8_status))
-        break;
+      if (!f8_drain<ACT>(eb, cols, ep, acc, use_res, rows_in, lane, m_box, args.M, nbase, N, &tmOut, abort_flag)) break;
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -559,6 +648,27 @@ __device__ __forceinline__ uint32_t f8_codes2(float lo, float hi, float inv) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// Largest finite magnitude of 8 elements.
+__device__ __forceinline__ float f8_amax8(const float (&f)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[e]));
+  return m;
+}
+__device__ __forceinline__ uint2 f8_codes8(const float (&f)[8], float inv) {
+  return make_uint2(f8_codes2(f[0], f[1], inv) | (f8_codes2(f[2], f[3], inv) << 16),
+                    f8_codes2(f[4], f[5], inv) | (f8_codes2(f[6], f[7], inv) << 16));
+}
+// The same on packed bf16: magnitudes compare as integers, and only a vector that holds an infinity or NaN (bits of at
+// least 0x7f80) takes the general form.
+__device__ __forceinline__ uint32_t f8_packed_max(const uint4& v) {
+  const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  return max(m & 0xffffu, m >> 16);
+}
+__device__ __forceinline__ uint32_t f8_codes2_finite(uint32_t pair, float inv) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(bf16_lo(pair) * inv, bf16_hi(pair) * inv), __NV_SATFINITE, __NV_E4M3);
+}
+
 template <typename T>
 __device__ __forceinline__ void f8_load8(const T* p, float (&f)[8]);
 template <>
@@ -585,29 +695,47 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const T* __restr
   const int kb = (int)((uint32_t)unit - group * (uint32_t)kblocks);
   const int k = kb * 128 + 8 * sub;
   const bool in = k < K;  // K is a multiple of 16
-  float f[R][8];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
-    if (in && r0 + i < rows) f8_load8(x + (r0 + i) * ld + k, f[i]);
-  }
   const uint32_t half = 0xffffu << (threadIdx.x & 16);
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (r0 + i >= rows) break;  // the same for the 16 lanes
-    float m = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[i][e]));
+  auto emit = [&](int i, float m, auto codes) {  // row r0 + i: the block's maximum, its scale, this lane's codes
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
     const uint32_t byte = f8_scale_of(m);
     if (sub == 0) sf[(r0 + i) * ldsf + kb] = (unsigned char)byte;
-    if (in) {
-      const float inv = f8_inverse(byte);
-      *reinterpret_cast<uint2*>(q + (r0 + i) * K + k) =
-          make_uint2(f8_codes2(f[i][0], f[i][1], inv) | (f8_codes2(f[i][2], f[i][3], inv) << 16),
-                     f8_codes2(f[i][4], f[i][5], inv) | (f8_codes2(f[i][6], f[i][7], inv) << 16));
+    if (in) *reinterpret_cast<uint2*>(q + (r0 + i) * K + k) = codes(f8_inverse(byte));
+  };
+  if constexpr (sizeof(T) == 2) {
+    uint4 v[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      v[i] = in && r0 + i < rows ? ldg_nc_u4(x + (r0 + i) * ld + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= rows) break;  // the same for the 16 lanes
+      const uint32_t m = f8_packed_max(v[i]);
+      const bool finite = m < 0x7f80u;
+      float f[8], amax = __uint_as_float(m << 16);
+      if (!finite) {
+        unpack8(v[i], f);
+        amax = f8_amax8(f);
+      }
+      emit(i, amax, [&](float inv) {
+        if (!finite) return f8_codes8(f, inv);
+        return make_uint2(f8_codes2_finite(v[i].x, inv) | (f8_codes2_finite(v[i].y, inv) << 16),
+                          f8_codes2_finite(v[i].z, inv) | (f8_codes2_finite(v[i].w, inv) << 16));
+      });
+    }
+  } else {
+    float f[R][8];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+      if (in && r0 + i < rows) f8_load8(x + (r0 + i) * ld + k, f[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= rows) break;
+      emit(i, f8_amax8(f[i]), [&](float inv) { return f8_codes8(f[i], inv); });
     }
   }
 }
@@ -628,8 +756,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles_kernel(const T* __rest
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[p][e] = 0.f;
     if (k < K && r < rows) f8_load8(x + r * ld + k, f[p]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, f8_finite_abs(f[p][e]));
+    m = fmaxf(m, f8_amax8(f[p]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -644,9 +771,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles_kernel(const T* __rest
   for (int p = 0; p < 8; ++p) {
     const int64_t r = r0 + 16 * p + slot;
     if (k < K && r < rows)
-      *reinterpret_cast<uint2*>(q + r * K + k) =
-          make_uint2(f8_codes2(f[p][0], f[p][1], inv) | (f8_codes2(f[p][2], f[p][3], inv) << 16),
-                     f8_codes2(f[p][4], f[p][5], inv) | (f8_codes2(f[p][6], f[p][7], inv) << 16));
+      *reinterpret_cast<uint2*>(q + r * K + k) = f8_codes8(f[p], inv);
   }
 }
 
@@ -671,6 +796,32 @@ static int launch_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t
     fp8_quantize_tiles_kernel<T><<<dim3((unsigned)kblocks, (unsigned)rb), 256, 0, st>>>(xp, ld, qp, sp, ldsf, rows, (int)K);
   }
   SANA_LAUNCH_CHECK("fp8_quantize kernel");
+  return SANA_OK;
+}
+
+template <int ACT>
+static int launch_gemm_fp8(bool pair, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
+                           const CUtensorMap& tmRes, F8Args& a, cudaStream_t st) {
+  a.tiles_m = (int)ceil_div(a.M, pair ? 256 : S8_BM);
+  a.tiles_n = (int)ceil_div(a.N, pair ? P8_BN : S8_BN);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
+  static OncePerDevice once;
+  if (once.first_time()) {
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM_BYTES);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_fp8_tc_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S8_SMEM_BYTES);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_fp8)");
+  }
+  if (pair) {
+    const int64_t max_clusters = sm_count() / 2;
+    const int grid = (int)(2 * (tiles < max_clusters ? tiles : max_clusters));
+    gemm_fp8_pair_kernel<ACT><<<grid, P8_THREADS, P8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
+  } else {
+    const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
+    gemm_fp8_tc_kernel<ACT><<<grid, F8_THREADS, S8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
+  }
+  SANA_LAUNCH_CHECK("gemm_fp8 kernel");
   return SANA_OK;
 }
 
@@ -733,35 +884,12 @@ extern "C" int sana_gemm_fp8(const void* Aq, const void* sfa, int64_t ldsfa, int
   if (rc) return rc;
   rc = make_tmap_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, Wq, N, K, K, 128, F8_BK);
   if (rc) return rc;
-  if (pair) {
-    static OncePerDevice once;
-    if (once.first_time()) {
-      cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM_BYTES);
-      if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_fp8_pair)");
-    }
-    a.tiles_m = (int)ceil_div(M, 256);
-    a.tiles_n = (int)ceil_div(N, P8_BN);
-    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-    SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
-    const int64_t max_clusters = sm_count() / 2;
-    const int grid = (int)(2 * (tiles < max_clusters ? tiles : max_clusters));
-    gemm_fp8_pair_kernel<<<grid, F8_THREADS, P8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
-    SANA_LAUNCH_CHECK("gemm_fp8_pair kernel");
-    return SANA_OK;
+  switch (p.act) {
+    case 0: return launch_gemm_fp8<0>(pair, tmA, tmB, tmOut, tmRes, a, st);
+    case 1: return launch_gemm_fp8<1>(pair, tmA, tmB, tmOut, tmRes, a, st);
+    case 2: return launch_gemm_fp8<2>(pair, tmA, tmB, tmOut, tmRes, a, st);
+    default: return launch_gemm_fp8<3>(pair, tmA, tmB, tmOut, tmRes, a, st);
   }
-  static OncePerDevice once;
-  if (once.first_time()) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S8_SMEM_BYTES);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_fp8_tc)");
-  }
-  a.tiles_m = (int)ceil_div(M, S8_BM);
-  a.tiles_n = (int)ceil_div(N, S8_BN);
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
-  const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
-  gemm_fp8_tc_kernel<<<grid, F8_THREADS, S8_SMEM_BYTES, st>>>(tmA, tmB, tmOut, tmRes, a);
-  SANA_LAUNCH_CHECK("gemm_fp8_tc kernel");
-  return SANA_OK;
 }
 
 extern "C" int sana_gemm_fp8_take_device_status(int* status_out) {
