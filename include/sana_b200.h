@@ -277,6 +277,8 @@ int sana_la_decay_step(const void* q, int64_t ldq, const void* k, int64_t ldk, c
                   const float* log_decay,
                        float* state, int64_t pool, const int32_t* slots, void* out, int64_t ldo, int64_t B, int64_t H,
                        int64_t Hk, int64_t D, float scale, int relu, float eps, int dtype, void* stream);
+/* Soft-error word of the tcgen05 kernels of sana_la_decay, whose waits are bounded (as sana_la_rope_take_device_status). */
+int sana_la_decay_take_device_status(int* status_out);
 
 /* ---------------------------------------------------------------------------------------
  * 3x3 depthwise conv + bias + SiLU-GLU on channels-last rows:

@@ -22,31 +22,12 @@
 // A sequence is split over CTAs into segments when there are fewer heads than the GPU has room for: a first launch
 // computes what each segment adds to the state, and each CTA of the second combines those of the segments before its
 // own, in order (nothing depends on the order in which CTAs run).
-#include "la_plan.cuh"
-#include "tc_common.cuh"
+#include "la_decay.cuh"
 
 namespace sana {
 
 constexpr int LD_C = 64;  // tokens per chunk, bf16
 constexpr int LD_CF = 32;  // fp32
-
-struct LdArgs {
-  const void *q, *k, *v;
-  int64_t ldq, ldk, ldv;
-  const float* log_decay;    // [H]
-  const float* prior;        // [B, H, D+1, D] or null
-  const int* lengths;        // [B] or null
-  float* partial;            // [B, nseg - 1, H, D+1, D]
-  float* state;              // [B, H, D+1, D]
-  void* out;
-  int64_t ldo;
-  int N, H, group;           // group = query heads per key/value head
-  int seg_len, nseg;
-  float scale, eps;
-  int relu, normalise;
-};
-
-__device__ __forceinline__ float ld_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
 
 __device__ __forceinline__ void ld_cp16(uint32_t dst, const void* src, bool valid) {
   const int sz = valid ? 16 : 0;
@@ -60,19 +41,9 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ld_relu4(uint32_t (&r)[4]) {  // a NaN stays one
+__device__ __forceinline__ void ld_relu4(uint32_t (&r)[4]) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const __nv_bfloat162 x = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&r[e]), __floats2bfloat162_rn(0.f, 0.f));
-    r[e] = *reinterpret_cast<const uint32_t*>(&x);
-  }
-}
-// the bf16 pair nearest (a, b), and what it leaves of them
-__device__ __forceinline__ uint32_t ld_split(float& a, float& b) {
-  const uint32_t p = pack_bf16(a, b);
-  a -= bf16_lo(p);
-  b -= bf16_hi(p);
-  return p;
+  for (int e = 0; e < 4; ++e) r[e] = ld_relu2(r[e]);
 }
 
 template <int D>
@@ -173,7 +144,7 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
     for (int r = 0; r < seg; ++r) {
       const int end = min((r + 1) * a.seg_len, len);
       if (end == min(r * a.seg_len, len)) break;  // past the sequence: these segments hold nothing
-      add(a.partial + (((int64_t)b * (a.nseg - 1) + r) * a.H + h) * per, ld_power(gl, n_begin - end));
+      add(a.partial + (((int64_t)b * a.npart + r) * a.H + h) * per, ld_power(gl, n_begin - end));
     }
   }
   auto publish_z = [&]() {  // the key sum into shared memory: the three terms are rows 0, 1, 2 = lanes 4 g
@@ -398,7 +369,7 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
   if (!active) return;
 
   if (!OUT || seg == a.nseg - 1) {
-    float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * (a.nseg - 1) + seg) * a.H + h) * per;
+    float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
     float* r = dst + (int64_t)(16 * wh + g) * D + c2;
 #pragma unroll
     for (int n = 0; n < 2 * KT; ++n) {
@@ -458,7 +429,7 @@ __global__ void __launch_bounds__(256) la_decay_f32_kernel(const LdArgs a) {
       for (int r = 0; r < seg; ++r) {
         const int end = min((r + 1) * a.seg_len, len);
         if (end == min(r * a.seg_len, len)) break;
-        x = fmaf(ld_power(gl, n_begin - end), a.partial[(((int64_t)b * (a.nseg - 1) + r) * a.H + h) * per + i], x);
+        x = fmaf(ld_power(gl, n_begin - end), a.partial[(((int64_t)b * a.npart + r) * a.H + h) * per + i], x);
       }
     }
     ss[(i / D) * ROW + i % D] = x;
@@ -550,7 +521,7 @@ __global__ void __launch_bounds__(256) la_decay_f32_kernel(const LdArgs a) {
   }
   __syncthreads();
   if (!OUT || seg == a.nseg - 1) {
-    float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * (a.nseg - 1) + seg) * a.H + h) * per;
+    float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
     for (int i = tid; i < (D + 1) * D; i += 256) dst[i] = ss[(i / D) * ROW + i % D];
   }
   if (OUT) {
@@ -677,10 +648,25 @@ static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, in
   *nseg = (int)ceil_div(N, (int64_t)*seg_len);
 }
 
+constexpr int64_t LD_TC_TOKENS = 65;  // shortest sequences the tcgen05 kernels take
+
+template <int D>
+static void ld_any_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, int* nseg, int* npart) {
+  if (dtype == SANA_BF16 && N >= LD_TC_TOKENS) {
+    const LdPlan p = ld_tc_plan(B, N, H, D, npart);
+    *seg_len = p.seg_len;
+    *nseg = p.nseg;
+  } else {
+    ld_plan<D>(B, N, H, dtype, seg_len, nseg);
+    *npart = *nseg - 1;
+  }
+}
+
 template <int D>
 static int launch_decay(LdArgs& a, int64_t B, int dtype, int64_t workspace_bytes, cudaStream_t st) {
-  ld_plan<D>(B, a.N, a.H, dtype, &a.seg_len, &a.nseg);
-  SANA_REQUIRE(workspace_bytes >= (int64_t)4 * B * (a.nseg - 1) * a.H * (D + 1) * D, "sana_la_decay: workspace too small");
+  ld_any_plan<D>(B, a.N, a.H, dtype, &a.seg_len, &a.nseg, &a.npart);
+  SANA_REQUIRE(workspace_bytes >= (int64_t)4 * B * a.npart * a.H * (D + 1) * D, "sana_la_decay: workspace too small");
+  if (dtype == SANA_BF16 && a.N >= LD_TC_TOKENS) return launch_decay_tc(a, B, D, st);
   if (dtype == SANA_BF16) {
     const dim3 grid((unsigned)ceil_div(a.H, Ld<D>::HG), (unsigned)a.nseg, (unsigned)B);
     if (a.nseg > 1) {
@@ -742,9 +728,9 @@ using namespace sana;
 
 extern "C" int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype) {
   if (B <= 0 || N <= 0 || N >= ((int64_t)1 << 30) || H <= 0 || !ld_head_dim(D) || (dtype != SANA_BF16 && dtype != SANA_F32)) return -1;
-  int len = 0, nseg = 1;
-  LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, &len, &nseg)));
-  return (int64_t)4 * B * (nseg - 1) * H * (D + 1) * D;
+  int len = 0, nseg = 1, npart = 0;
+  LD_DISPATCH(D, (ld_any_plan<HD>(B, N, H, dtype, &len, &nseg, &npart)));
+  return (int64_t)4 * B * npart * H * (D + 1) * D;
 }
 
 extern "C" int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* log_decay,
@@ -759,7 +745,7 @@ extern "C" int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t 
   SANA_REQUIRE(prior != state, "sana_la_decay: prior and state must be different buffers");
   SANA_REQUIRE(workspace || workspace_bytes == 0, "sana_la_decay: null workspace");
   LdArgs a = {q, k, v, ldq, ldk, ldv, log_decay, prior, lengths, static_cast<float*>(workspace), state, out, ldo, (int)N, (int)H,
-              (int)(H / Hk), 0, 0, scale, eps, relu ? 1 : 0, eps >= 0.f ? 1 : 0};
+              (int)(H / Hk), 0, 0, 0, scale, eps, relu ? 1 : 0, eps >= 0.f ? 1 : 0};
   LD_DISPATCH(D, return (launch_decay<HD>(a, B, dtype, workspace_bytes, static_cast<cudaStream_t>(stream))));
   return SANA_ERR_INVALID;
 }

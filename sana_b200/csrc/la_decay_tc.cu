@@ -1,0 +1,613 @@
+// Causal linear attention with a decay for each head, bf16, on the 5th-generation tensor cores (formulas in la_decay.cu).
+//
+// A CTA walks one token segment of one head in chunks of 128 tokens.  With v1 = [v ; 1] (the ones column makes the key sum
+// and the normaliser come out of the same products), w_t = lambda^(C-1-t), and S the state before the chunk:
+//
+//   scores  SC  = phi(Q) phi(K)^T                     M = 128 queries, N = 128 keys, K = D
+//   inter   O1  = phi(Q) S^T                          N = D + 16, K = D          row t is scaled by lambda^(t+1) at the end
+//   intra   O2  = (SC * lambda^(t-s), s <= t) V1      N = D + 16, K = 128        A operand in tensor memory, bf16
+//   state   dS^T = (w K)^T V1                         M = D key channels, N = D + 16, K = 128 tokens
+//
+// Every tile is [64-channel block][row][128 bytes], 128-byte swizzled, which serves as a K-major operand (rows = M or N)
+// and as an MN-major one (rows = K) alike: k and q are stored once and used both ways, and the bulk-tensor copies write
+// them in place (4-D views (channel, head, token, sample): channels past the head arrive as zeros).
+//
+// Roles: warps 0-3 keep the state (thread j: key channel j against all value channels, fp32 registers), join the chunk's
+// sum to it (S = lambda^C S + dS: one rounded multiply-add per chunk, since the tensor core truncates its sums), write it
+// as the bf16 operand of O1, and finish the outputs; warps 4-7 decay and mask the scores; the next 4 or 8 warps weight the
+// keys, apply ReLU in place and put the ones column back beside v; one warp issues the products, one the copies.
+// The weighted k is split into NT bf16 terms: 3 where the state that leaves the kernel is exact to fp32 (2^-24), 2 where
+// it only serves the outputs (2^-16, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
+// rows of one product, and the state warps add them; an instruction costs 42 + N / 2 cycles whatever part of its rows
+// is used.  All waits are bounded.
+#include "la_decay.cuh"
+
+namespace sana {
+
+__device__ int g_ld_status = 0;
+
+constexpr int LT_C = 128;
+constexpr int LT_BLK = LT_C * 128;  // one 64-channel block of a token tile
+
+template <int D, int NT, bool OUT>
+struct Lt {
+  static constexpr int NV = D + 16;                      // value columns: D channels, the ones column, padding
+  static constexpr int KB = (D + 63) / 64, VB = (NV + 63) / 64;
+  static constexpr int LW = D <= 64 ? 4 : 8;             // warps that weight the keys: thread = token (and half of its channels)
+  static constexpr int LT = 32 * LW;
+  static constexpr bool WIDE = D >= 80;
+  static constexpr int THREADS = 32 * (8 + LW + (WIDE ? 4 : 2));  // wide heads: whole warpgroups, for the register split
+  static constexpr bool STACK = D <= 32;                 // terms of the weighted k side by side, 32 channels apart
+  static constexpr int MMAS = STACK ? 1 : NT;            // products per 16 tokens of the state update
+  static constexpr int KTILE = KB * LT_BLK, VTILE = VB * LT_BLK;
+  static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
+  static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
+  static constexpr int OFF_W = 0;                        // weighted k (followed by v: with one block of 64 channels, rows
+  static constexpr int OFF_V = OFF_W + WTILE;            // 64 .. 127 of the product read there and are not used)
+  static constexpr int OFF_K = OFF_V + VTILE;
+  static constexpr int OFF_Q = OFF_K + KTILE;
+  static constexpr int OFF_S = OFF_Q + (OUT ? KTILE : 0);
+  static constexpr int OFF_X = OFF_S + (OUT ? VB * STATE_BLK : 0);  // sums of the second and third term, [2][D+1][32]
+  static constexpr int OFF_POW = OFF_X + (STACK ? (NT - 1) * (D + 1) * 32 * 4 : 0);
+  static constexpr int OFF_BAR = OFF_POW + 4 * (LT_C + 4);
+  static constexpr int BYTES = OFF_BAR + 8 * 24;
+  static constexpr int COL_SC = 0, COL_O2 = 64;          // O2 starts inside the scores: they are all read by then
+  static constexpr int COL_O1 = 64 + NV > 128 ? 64 + NV : 128;
+  static constexpr int COL_DS = OUT ? COL_O1 + NV : 0;
+  static constexpr int COLS = COL_DS + NV;
+  static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int CTAS = TMEM_COLS <= 256 && 2 * (BYTES + 1024) <= 228 * 1024 && D <= 32 ? 2 : 1;  // resident per SM
+  // D = f32 (bit 4), A = B = bf16 (7, 10), transposes (MN-major) at 15 / 16, N >> 3 at 17, M >> 4 at 24
+  static constexpr uint32_t BASE = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+  static constexpr uint32_t ID_SC = BASE | ((128u >> 3) << 17);
+  static constexpr uint32_t ID_O = BASE | (1u << 16) | ((uint32_t)(NV >> 3) << 17);
+  static constexpr uint32_t ID_DS = BASE | (1u << 15) | (1u << 16) | ((uint32_t)(NV >> 3) << 17);
+  static_assert(COLS <= 512 && BYTES <= 232448, "budgets");
+};
+
+__device__ __forceinline__ uint64_t lt_desc_mn(uint32_t saddr, uint32_t block_stride_bytes) {
+  const uint32_t lo = ((saddr >> 4) & 0x3FFFu) | ((block_stride_bytes >> 4) << 16);
+  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
+}
+__device__ __forceinline__ void lt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void lt_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ uint32_t lt_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  return r;
+}
+
+template <int D, int NT, bool OUT>
+__global__ void __launch_bounds__(Lt<D, NT, OUT>::THREADS, Lt<D, NT, OUT>::CTAS) 
+la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ CUtensorMap tmQ, const LdArgs a) {
+  using T = Lt<D, NT, OUT>;
+  constexpr int C = LT_C, NV = T::NV, LW = T::LW;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t sm = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if ((sm & 1023u) != 0u) {  // uniform over the CTA: nothing has been set up yet
+    if (tid == 0) atomicExch(&g_ld_status, 9);
+    return;
+  }
+  float* pow_s = reinterpret_cast<float*>(smem + T::OFF_POW);
+  // barriers: raw tiles have landed / tiles are ready (k: weighted, by halves of 64 tokens) / tiles are free; scores ready,
+  // decayed scores ready, chunk sum ready / read, state operand ready / read, outputs ready / read
+  const uint32_t bar = sm + T::OFF_BAR;
+  const uint32_t kraw = bar, qraw = bar + 8, vraw = bar + 16, wfull = bar + 24 /* 2 */, qfull = bar + 40, vfull = bar + 48;
+  const uint32_t kempty = bar + 56, qempty = bar + 64, vempty = bar + 72, wempty = bar + 80 /* 2 */;
+  const uint32_t scready = bar + 96, dsready = bar + 104, sopread = bar + 112, oready = bar + 120;
+  const uint32_t pready = bar + 128, dsread = bar + 136, sopready = bar + 144, oread = bar + 152;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 160);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 164);
+
+  const int h = blockIdx.x, seg = blockIdx.y, b = blockIdx.z;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const int seg_begin = seg * a.seg_len, seg_end = min(a.N, seg_begin + a.seg_len);
+  const int n_begin = min(seg_begin, len), n_end = min(seg_end, len);
+  const int chunks = (n_end - n_begin + C - 1) / C;
+  const float gl = a.log_decay[h];
+  const int64_t row0 = (int64_t)b * a.N;
+  const int64_t per = (int64_t)(D + 1) * D;
+
+  if (tid == 0) {
+    for (int i = 0; i < 20; ++i) mbar_init(bar + 8 * i, i >= 16 ? 4 : 1);
+    mbar_init(wfull, LW / 2);
+    mbar_init(wfull + 8, LW / 2);
+    mbar_init(qfull, LW);
+    mbar_init(vfull, LW);
+    if (!OUT) mbar_init(kempty, LW);  // no scores: k is free once it has been weighted
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 160), "r"((uint32_t)T::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  for (int i = tid; i <= C; i += T::THREADS) pow_s[i] = ld_power(gl, i);
+  // the ones column of v1 and its padding, once: token t, channels D .. D + 15 = two 16-byte pieces
+  for (int i = tid; i < 2 * C; i += T::THREADS) {
+    const int t = i >> 1, ch = D / 8 + (i & 1);
+    *reinterpret_cast<uint4*>(smem + T::OFF_V + (ch >> 3) * LT_BLK + t * 128 + (((ch & 7) ^ (t & 7)) << 4)) =
+        make_uint4((i & 1) ? 0u : 0x3f80u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Wide heads: 640 threads start with 96 registers each; the state warps, which hold a row of the state, take over what
+  // the others give up: 128 x 192 + 128 x 64 + 256 x 72 + 128 x 80 = 61 440 = 640 x 96
+  if (warp < 4) {
+    // ------------------------------- state and outputs ---------------------------------
+    if constexpr (T::WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int j = tid;            // key channel (state)
+    const int t = tid;            // query of the chunk (outputs)
+    const bool jin = j < D, warp_in = warp * 32 < D;
+    float S[D + 1];
+#pragma unroll
+    for (int i = 0; i <= D; ++i) S[i] = 0.f;
+    if (OUT && jin) {  // the state before this segment
+      auto add = [&](const float* src, float f) {
+#pragma unroll
+        for (int i = 0; i <= D; ++i) S[i] = fmaf(f, __ldg(src + i * D + j), S[i]);
+      };
+      if (a.prior) add(a.prior + ((int64_t)b * a.H + h) * per, ld_power(gl, n_begin));
+      for (int r = 0; r < seg; ++r) {
+        const int end = min((r + 1) * a.seg_len, len);
+        if (end == min(r * a.seg_len, len)) break;  // past the sequence: these segments hold nothing
+        add(a.partial + (((int64_t)b * a.npart + r) * a.H + h) * per, ld_power(gl, n_begin - end));
+      }
+      if (a.npart > 0 && seg == a.nseg - 1) {  // the exact sums of all segments are known: the state after the last token
+        float* dst = a.state + ((int64_t)b * a.H + h) * per;
+        const float* src = a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
+        const float f = ld_power(gl, n_end - n_begin);
+#pragma unroll
+        for (int i = 0; i <= D; ++i) dst[i * D + j] = fmaf(f, S[i], n_end > n_begin ? __ldg(src + i * D + j) : 0.f);
+      }
+    }
+    // row j of the state operand: value channels 16 c .. + 15 as two 16-byte pieces
+    auto write_operand = [&]() {
+      if (jin) {
+        unsigned char* row = smem + T::OFF_S + j * 128;
+#pragma unroll
+        for (int c = 0; c < NV / 8; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * c + 2 * e;
+            w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? pack_bf16(S[D], 0.f) : 0u;
+          }
+          *reinterpret_cast<uint4*>(row + (c >> 3) * T::STATE_BLK + (((c & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sopready);
+    };
+    if (OUT && chunks > 0) write_operand();
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t ph = (uint32_t)(c & 1);
+      const int n0 = n_begin + c * C, nv = min(C, n_end - n0);
+      if (!mbar_wait(dsready, ph, abort_flag, 1, &g_ld_status)) { ok = false; break; }
+      tcgen05_fence_after();
+      if constexpr (T::STACK) {  // warps 1 .. NT - 1 hold the sums of the lesser terms, lane = key channel
+        float* x = reinterpret_cast<float*>(smem + T::OFF_X);
+        if (warp > 0 && warp < NT) {
+#pragma unroll
+          for (int g = 0; g < D / 16; ++g) {
+            uint32_t d[16];
+            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[((warp - 1) * (D + 1) + 16 * g + e) * 32 + lane] = __uint_as_float(d[e]);
+          }
+          const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
+          tmem_ld_wait();
+          x[((warp - 1) * (D + 1) + D) * 32 + lane] = __uint_as_float(d);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (warp == 0) {
+          const float whole = pow_s[nv];
+          auto join = [&](int i, uint32_t d) {
+            float r = x[i * 32 + lane];
+            if (NT == 3) r += x[(D + 1 + i) * 32 + lane];
+            S[i] = fmaf(whole, S[i], __uint_as_float(d) + r);
+          };
+#pragma unroll
+          for (int g = 0; g < D / 16; ++g) {
+            uint32_t d[16];
+            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) join(16 * g + e, d[e]);
+          }
+          const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
+          tmem_ld_wait();
+          join(D, d);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the scratch is free again
+      } else if (warp_in) {
+        const float whole = pow_s[nv];
+#pragma unroll
+        for (int g = 0; g < D / 16; ++g) {
+          uint32_t d[16];
+          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[16 * g + e] = fmaf(whole, S[16 * g + e], __uint_as_float(d[e]));
+        }
+        const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
+        tmem_ld_wait();
+        S[D] = fmaf(whole, S[D], __uint_as_float(d));
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dsread);
+      if (OUT) {
+        if (c + 1 < chunks) {
+          if (!mbar_wait(sopread, ph, abort_flag, 2, &g_ld_status)) { ok = false; break; }
+          write_operand();
+        }
+        if (!mbar_wait(oready, ph, abort_flag, 3, &g_ld_status)) { ok = false; break; }
+        tcgen05_fence_after();
+        const float f = pow_s[t + 1];
+        float m = a.scale;
+        if (a.normalise) {
+          const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D)), d2 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O2 + D));
+          tmem_ld_wait();
+          m = 1.f / (fmaf(f, __uint_as_float(d1), __uint_as_float(d2)) + a.eps);
+        }
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row0 + n0 + t) * a.ldo + (int64_t)h * D;
+#pragma unroll
+        for (int g = 0; g < D / 16; ++g) {
+          uint32_t x[16], y[16], w[8];
+          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O1 + 16 * g), x);
+          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O2 + 16 * g), y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = pack_bf16(fmaf(f, __uint_as_float(x[2 * e]), __uint_as_float(y[2 * e])) * m,
+                             fmaf(f, __uint_as_float(x[2 * e + 1]), __uint_as_float(y[2 * e + 1])) * m);
+          if (t < nv) {
+            *reinterpret_cast<uint4*>(dst + 16 * g) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + 16 * g + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(oread);
+      }
+    }
+    if (ok && jin && (!OUT || (a.npart == 0 && seg == a.nseg - 1))) {
+      float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
+#pragma unroll
+      for (int i = 0; i <= D; ++i) dst[i * D + j] = S[i];
+    }
+  } else if (warp < 8) {
+    // ------------------------------- scores --------------------------------------------
+    if constexpr (T::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (OUT) {
+      const int w = warp - 4;
+      const uint32_t sc = tmem + ((uint32_t)(w * 32) << 16) + (uint32_t)T::COL_SC;
+      for (int c = 0; c < chunks; ++c) {
+        if (!mbar_wait(scready, (uint32_t)(c & 1), abort_flag, 4, &g_ld_status)) break;
+        tcgen05_fence_after();
+#pragma unroll 1
+        for (int blk = 0; blk < 4; ++blk) {  // keys 32 blk .. + 31; the bf16 pairs go over scores that have been read
+          uint32_t p[16];
+          if (blk > w) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = 0u;
+          } else {
+            uint32_t x[32];
+            tmem_ld_32x32(sc + (uint32_t)(32 * blk), x);
+            tmem_ld_wait();
+            if (blk < w) {  // every key lies before every query: lambda^(t - s) = lambda^(t - s0 - 31) lambda^(31 - k)
+              const float f = pow_s[32 * (w - blk) + lane - 31];
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                p[e] = pack_bf16(__uint_as_float(x[2 * e]) * (f * pow_s[31 - 2 * e]), __uint_as_float(x[2 * e + 1]) * (f * pow_s[30 - 2 * e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int d0 = lane - 2 * e, d1 = d0 - 1;  // t - s
+                const float p0 = d0 >= 0 ? __uint_as_float(x[2 * e]) * pow_s[max(d0, 0)] : 0.f;
+                const float p1 = d1 >= 0 ? __uint_as_float(x[2 * e + 1]) * pow_s[max(d1, 0)] : 0.f;
+                p[e] = pack_bf16(p0, p1);
+              }
+            }
+          }
+          lt_st16(sc + (uint32_t)(16 * blk), p);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pready);
+      }
+      // rows of the segment past the sequence are zeros
+      const int z0 = max(seg_begin, n_end);
+      for (int64_t i = tid - 128; i < (int64_t)max(0, seg_end - z0) * (D / 8); i += 128) {
+        const int t = z0 + (int)(i / (D / 8)), ch = (int)(i % (D / 8));
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 8 * ch) =
+            make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  } else if (warp < 8 + LW) {
+    // ------------------------------- weighted keys, features, ones column ----------------
+    if constexpr (T::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int row = (tid - 256) & 127, part = (tid - 256) >> 7;  // token of the chunk; which of the interleaved 16-byte pieces
+    constexpr int PARTS = T::LT / 128;
+    const bool relu = a.relu != 0;
+    const uint32_t wbar = 8u * (uint32_t)(row >> 6);  // warp-uniform: the half of the tokens
+    unsigned char* krow = smem + T::OFF_K + row * 128;
+    unsigned char* qrow = smem + T::OFF_Q + row * 128;
+    unsigned char* vrow = smem + T::OFF_V + row * 128;
+    auto piece = [&](int ch) -> uint32_t { return (uint32_t)((ch >> 3) * LT_BLK + (((ch & 7) ^ (row & 7)) << 4)); };
+    auto relu4 = [&](uint4 r) { return make_uint4(ld_relu2(r.x), ld_relu2(r.y), ld_relu2(r.z), ld_relu2(r.w)); };
+    auto publish = [&](uint32_t full) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+    };
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t ph = (uint32_t)(c & 1);
+      const int nv = min(C, n_end - (n_begin + c * C));
+      const bool live = row < nv;
+      if (!mbar_wait(kraw, ph, abort_flag, 5, &g_ld_status)) break;
+      if (!mbar_wait(wempty + wbar, ph ^ 1u, abort_flag, 6, &g_ld_status)) break;
+      const float wt = live ? pow_s[nv - 1 - row] : 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8 / PARTS; ++i) {
+        const int ch = i * PARTS + part;
+        uint4* kp = reinterpret_cast<uint4*>(krow + piece(ch));
+        uint4 r = *kp;
+        if (relu) {
+          r = relu4(r);
+          if (OUT) *kp = r;
+        }
+        if (!live) r = make_uint4(0u, 0u, 0u, 0u);  // whatever lies behind the sequence
+        uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        float x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = bf16_lo(w[e]) * wt, y[e] = bf16_hi(w[e]) * wt;
+#pragma unroll
+        for (int s = 0; s < NT; ++s) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = s + 1 < NT ? ld_split(x[e], y[e]) : pack_bf16(x[e], y[e]);
+          const uint32_t at = T::STACK ? piece(ch + 4 * s) : (uint32_t)(s * T::KTILE) + piece(ch);
+          *reinterpret_cast<uint4*>(smem + T::OFF_W + row * 128 + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      publish(wfull + wbar);
+      if (!OUT) {
+        if (lane == 0) mbar_arrive(kempty);
+      } else {
+        if (!mbar_wait(qraw, ph, abort_flag, 7, &g_ld_status)) break;
+        if (relu) {
+#pragma unroll
+          for (int i = 0; i < D / 8 / PARTS; ++i) {
+            uint4* p = reinterpret_cast<uint4*>(qrow + piece(i * PARTS + part));
+            *p = relu4(*p);
+          }
+        }
+        publish(qfull);
+      }
+      if (!mbar_wait(vraw, ph, abort_flag, 8, &g_ld_status)) break;
+      if (!live) {  // rows behind the sequence meet zero weights: they must be finite
+#pragma unroll
+        for (int i = 0; i < D / 8 / PARTS; ++i) *reinterpret_cast<uint4*>(vrow + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vrow + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
+      publish(vfull);
+    }
+  } else {
+    // ------------------------------- products -------------------------------------------
+    if constexpr (T::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8 + LW) {  // the whole warp waits, one elected lane issues
+      const uint32_t Wu = sm + T::OFF_W, Vu = sm + T::OFF_V, Ku = sm + T::OFF_K, Qu = sm + T::OFF_Q, Su = sm + T::OFF_S;
+      const uint64_t vdesc = lt_desc_mn(Vu, LT_BLK), sdesc = lt_desc_mn(Su, T::STATE_BLK);
+      auto wait = [&](uint32_t bb, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bb, parity, abort_flag, code, &g_ld_status));
+      };
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t ph = (uint32_t)(c & 1);
+        if (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10)) break;
+        if (OUT) {
+          if (!wait(qfull, ph, 11) || !wait(oread, ph ^ 1u, 12)) break;  // the previous outputs lie over the scores
+          tcgen05_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16(tmem + T::COL_SC, make_smem_desc(Qu + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)),
+                        make_smem_desc(Ku + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), T::ID_SC, k != 0 ? 1u : 0u);
+            umma_commit(scready);
+            umma_commit(kempty);
+          }
+          __syncwarp();
+        }
+        if (!wait(vfull, ph, 13) || !wait(dsread, ph ^ 1u, 14)) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int s = T::MMAS - 1; s >= 0; --s) {  // smallest term first
+              const uint64_t wdesc = lt_desc_mn(Wu + s * T::KTILE, LT_BLK);
+#pragma unroll
+              for (int k = 4 * half; k < 4 * half + 4; ++k)
+                umma_bf16(tmem + T::COL_DS, wdesc + (uint64_t)(128 * k), vdesc + (uint64_t)(128 * k), T::ID_DS,
+                          (half != 0 || s != T::MMAS - 1 || k != 0) ? 1u : 0u);
+            }
+            umma_commit(wempty + 8 * half);
+          }
+          umma_commit(dsready);
+          if (!OUT) umma_commit(vempty);
+        }
+        __syncwarp();
+        if (!OUT) continue;
+        if (!wait(sopready, ph, 15)) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qu + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
+                      T::ID_O, k != 0 ? 1u : 0u);
+          umma_commit(qempty);
+          umma_commit(sopread);
+        }
+        __syncwarp();
+        if (!wait(pready, ph, 16)) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < C / 16; ++k)
+            lt_mma_ts(tmem + T::COL_O2, tmem + T::COL_SC + 8u * k, vdesc + (uint64_t)(128 * k), T::ID_O, k != 0 ? 1u : 0u);
+          umma_commit(vempty);
+          umma_commit(oready);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 9 + LW && lane == 0) {  // copies
+      const int hk = h / a.group;
+      auto copy = [&](uint32_t dst, const CUtensorMap* tm, uint32_t full, int head, int n0) {
+        mbar_expect_tx(full, (uint32_t)T::KTILE);
+#pragma unroll
+        for (int i = 0; i < T::KB; ++i)
+          asm volatile(
+              "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+              ::"r"(dst + i * LT_BLK), "l"(tm), "r"(full), "r"(64 * i), "r"(head), "r"(n0), "r"(b)
+              : "memory");
+      };
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t ph = (uint32_t)(c & 1);
+        const int n0 = n_begin + c * C;
+        if (!mbar_wait(kempty, ph ^ 1u, abort_flag, 17, &g_ld_status)) break;
+        copy(sm + T::OFF_K, &tmK, kraw, hk, n0);
+        if (OUT) {
+          if (!mbar_wait(qempty, ph ^ 1u, abort_flag, 18, &g_ld_status)) break;
+          copy(sm + T::OFF_Q, &tmQ, qraw, h, n0);
+        }
+        if (!mbar_wait(vempty, ph ^ 1u, abort_flag, 19, &g_ld_status)) break;
+        copy(sm + T::OFF_V, &tmV, vraw, hk, n0);
+      }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) {  // give products in flight time to end before tensor memory is freed
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {}
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)T::TMEM_COLS) : "memory");
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+struct LdMaps {
+  CUtensorMap k, v, q;
+};
+template <int D, int NT, bool OUT>
+static int lt_launch(const LdMaps& m, const LdArgs& a, int nseg, int64_t B, cudaStream_t st) {
+  using T = Lt<D, NT, OUT>;
+  static OncePerDevice once;
+  if (once.first_time()) {
+    cudaError_t e = cudaFuncSetAttribute(la_decay_tc_kernel<D, NT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::BYTES);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(la_decay_tc)");
+  }
+  la_decay_tc_kernel<D, NT, OUT><<<dim3((unsigned)a.H, (unsigned)nseg, (unsigned)B), T::THREADS, T::BYTES, st>>>(m.k, m.v, m.q, a);
+  SANA_LAUNCH_CHECK("la_decay_tc kernel");
+  return SANA_OK;
+}
+
+// One pass (the state in three terms) when the heads alone fill the GPU; else the sequence is cut: the first launch sums
+// every segment exactly, the second computes the outputs with two terms.  128-channel heads always take two (three terms
+// of the weighted k do not fit beside the other tiles).
+template <int D>
+static int lt_run(const LdArgs& a, int64_t B, cudaStream_t st) {
+  // (channel, head, token, sample) views of the column blocks; a box is 64 channels of 128 tokens of a head
+  LdMaps m;
+  const uint32_t box[4] = {64, 1, LT_C, 1};
+  auto view = [&](CUtensorMap* tm, const void* p, int64_t ld, int64_t heads) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)heads, (uint64_t)a.N, (uint64_t)B};
+    const uint64_t strides[3] = {(uint64_t)D * 2, (uint64_t)ld * 2, (uint64_t)ld * 2 * (uint64_t)a.N};
+    return make_tmap_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, p, dims, strides, box, true);
+  };
+  int rc = view(&m.k, a.k, a.ldk, a.H / a.group);
+  if (!rc) rc = view(&m.v, a.v, a.ldv, a.H / a.group);
+  if (!rc) rc = view(&m.q, a.q, a.ldq, a.H);
+  if (rc) return rc;
+  if constexpr (D < 128) {
+    if (a.npart == 0) return lt_launch<D, 3, true>(m, a, 1, B, st);
+  }
+  rc = lt_launch<D, 3, false>(m, a, a.nseg, B, st);
+  if (rc) return rc;
+  return lt_launch<D, 2, true>(m, a, a.nseg, B, st);
+}
+
+LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, int* npart) {
+  const int64_t units = B * H, slots = (int64_t)sm_count() * (D <= 32 ? 2 : 1), chunks = ceil_div(N, LT_C);
+  int64_t best = -1, best_len = chunks;
+  for (int64_t n = 1; n <= chunks && n <= 64; ++n) {
+    const int64_t len = ceil_div(chunks, n), real = ceil_div(chunks, len), waves = ceil_div(units * real, slots);
+    const bool two = real > 1 || D == 128;
+    const int64_t cost = waves * (two ? 16 * len + 20 + 2 * real : 12 * len + 10);  // tenths of a chunk
+    if (best < 0 || cost < best) best = cost, best_len = len;
+  }
+  LdPlan p;
+  p.seg_len = (int)(best_len * LT_C);
+  p.nseg = (int)ceil_div(N, (int64_t)p.seg_len);
+  *npart = (p.nseg > 1 || D == 128) ? p.nseg : 0;
+  return p;
+}
+
+int launch_decay_tc(LdArgs& a, int64_t B, int64_t D, cudaStream_t st) {
+  switch (D) {
+    case 16: return lt_run<16>(a, B, st);
+    case 32: return lt_run<32>(a, B, st);
+    case 48: return lt_run<48>(a, B, st);
+    case 64: return lt_run<64>(a, B, st);
+    case 80: return lt_run<80>(a, B, st);
+    case 96: return lt_run<96>(a, B, st);
+    case 112: return lt_run<112>(a, B, st);
+    default: return lt_run<128>(a, B, st);
+  }
+}
+
+}  // namespace sana
+
+extern "C" int sana_la_decay_take_device_status(int* status_out) {
+  if (!status_out) return sana::fail(SANA_ERR_INVALID, "sana_la_decay_take_device_status: null pointer");
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, sana::g_ld_status, sizeof(int));
+  if (e != cudaSuccess) return sana::cuda_status(e, "cudaMemcpyFromSymbol(g_ld_status)");
+  if (v != 0) {
+    int zero = 0;
+    e = cudaMemcpyToSymbol(sana::g_ld_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return sana::cuda_status(e, "cudaMemcpyToSymbol(g_ld_status)");
+  }
+  *status_out = v;
+  return SANA_OK;
+}

@@ -924,3 +924,10 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
                                               _dtype_code(q.dtype), _stream()), "sana_la_decay_step")
     counters.launches += 1
     return out
+
+
+def take_la_decay_device_status() -> int:
+    """Code recorded by a timed-out wait inside the tcgen05 kernels of :func:`la_decay` (0 = none).  Synchronises."""
+    v = C.c_int(0)
+    _lib.check(_lib.load().sana_la_decay_take_device_status(C.byref(v)), "sana_la_decay_take_device_status")
+    return int(v.value)

@@ -85,6 +85,7 @@ def run_case(B, N, H, D, dtype, Hk=None, relu=False, eps=None, prior=False, leng
     terms = state_tol(N, dtype) + 2 * D
     close(st, rs, ms, F32, "state", state_tol(N, dtype))
     close(out, ro, 2 * mo if eps is not None else mo, dtype, "out", terms)
+    assert ops.take_la_decay_device_status() == 0
     if lengths is not None:
         for b, m in enumerate(lengths):
             assert (out[b * N + max(0, m):(b + 1) * N] == 0).all()
