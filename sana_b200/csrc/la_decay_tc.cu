@@ -42,25 +42,37 @@ struct Lt {
   static constexpr int KTILE = KB * LT_BLK, VTILE = VB * LT_BLK;
   static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
   static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
+  static constexpr int X_BYTES = STACK ? NT * (D + 1) * 32 * 4 : 0;  // sums of the terms, [NT][D+1][32]
+  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 4) + (OUT ? 4 * 2 * LT_C : 0) + 8 * 32;
+  static constexpr int ONE_EACH = WTILE + VTILE + KTILE + (OUT ? KTILE : 0) + SCRATCH;
+  static constexpr int LIMIT = OUT && D <= 32 ? 113 * 1024 : 232448;  // two CTAs per SM, or one
+  // a second v tile hides the latency of its load behind the products that still need the first; then one for q
+  static constexpr int VBUF = ONE_EACH + VTILE <= LIMIT ? 2 : 1;
+  static constexpr int QBUF = OUT && ONE_EACH + (VBUF - 1) * VTILE + KTILE <= LIMIT ? 2 : 1;
   static constexpr int OFF_W = 0;                        // weighted k (followed by v: with one block of 64 channels, rows
   static constexpr int OFF_V = OFF_W + WTILE;            // 64 .. 127 of the product read there and are not used)
-  static constexpr int OFF_K = OFF_V + VTILE;
+  static constexpr int OFF_K = OFF_V + VBUF * VTILE;
   static constexpr int OFF_Q = OFF_K + KTILE;
-  static constexpr int OFF_S = OFF_Q + (OUT ? KTILE : 0);
-  static constexpr int OFF_X = OFF_S + (OUT ? VB * STATE_BLK : 0);  // sums of the second and third term, [2][D+1][32]
-  static constexpr int OFF_POW = OFF_X + (STACK ? (NT - 1) * (D + 1) * 32 * 4 : 0);
-  static constexpr int OFF_BAR = OFF_POW + 4 * (LT_C + 4);
-  static constexpr int BYTES = OFF_BAR + 8 * 24;
-  static constexpr int COL_SC = 0, COL_O2 = 64;          // O2 starts inside the scores: they are all read by then
-  static constexpr int COL_O1 = 64 + NV > 128 ? 64 + NV : 128;
+  static constexpr int OFF_S = OFF_Q + (OUT ? QBUF * KTILE : 0);
+  static constexpr int OFF_X = OFF_S + (OUT ? VB * STATE_BLK : 0);
+  static constexpr int OFF_POW = OFF_X + X_BYTES;        // powers behind 32 zeros
+  static constexpr int OFF_RS = OFF_POW + 4 * (32 + LT_C + 4);  // row sums of the scores, [2][128]
+  static constexpr int OFF_BAR = OFF_RS + (OUT ? 4 * 2 * LT_C : 0);
+  static constexpr int BYTES = OFF_BAR + 8 * 32;
+  // Scores in two halves of 64 keys.  O2 has columns of its own, except for 128 channels, where it starts inside the
+  // second half and the next chunk's scores wait until it has been read.
+  static constexpr bool ALIAS = 128 + 2 * NV + D > 512;
+  static constexpr int COL_SC = 0, COL_O2 = ALIAS ? 96 : 128;
+  static constexpr int COL_O1 = COL_O2 + D;
   static constexpr int COL_DS = OUT ? COL_O1 + NV : 0;
   static constexpr int COLS = COL_DS + NV;
   static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int CTAS = TMEM_COLS <= 256 && 2 * (BYTES + 1024) <= 228 * 1024 && D <= 32 ? 2 : 1;  // resident per SM
   // D = f32 (bit 4), A = B = bf16 (7, 10), transposes (MN-major) at 15 / 16, N >> 3 at 17, M >> 4 at 24
   static constexpr uint32_t BASE = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
-  static constexpr uint32_t ID_SC = BASE | ((128u >> 3) << 17);
-  static constexpr uint32_t ID_O = BASE | (1u << 16) | ((uint32_t)(NV >> 3) << 17);
+  static constexpr uint32_t ID_SC = BASE | ((64u >> 3) << 17);
+  static constexpr uint32_t ID_O1 = BASE | (1u << 16) | ((uint32_t)(NV >> 3) << 17);
+  static constexpr uint32_t ID_O2 = BASE | (1u << 16) | ((uint32_t)(D >> 3) << 17);
   static constexpr uint32_t ID_DS = BASE | (1u << 15) | (1u << 16) | ((uint32_t)(NV >> 3) << 17);
   static_assert(COLS <= 512 && BYTES <= 232448, "budgets");
 };
@@ -91,6 +103,25 @@ __device__ __forceinline__ uint32_t lt_ld1(uint32_t taddr) {
   return r;
 }
 
+// Bounded wait like mbar_wait, by all lanes of a warp and with the plain poll: the suspend hint of mbar_wait puts the warp
+// to sleep in steps, up to a microsecond past the arrival, and a chunk passes through eight waits in a row.
+__device__ __forceinline__ bool lt_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (mbar_try_wait_poll(bar, parity)) return true;
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (!mbar_try_wait_poll(bar, parity)) {
+    if ((++spins & 255u) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > TC_WAIT_LIMIT_CYCLES) {
+        *abort_flag = code;
+        atomicExch(&g_ld_status, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 template <int D, int NT, bool OUT>
 __global__ void __launch_bounds__(Lt<D, NT, OUT>::THREADS, Lt<D, NT, OUT>::CTAS) 
 la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -104,16 +135,18 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (tid == 0) atomicExch(&g_ld_status, 9);
     return;
   }
-  float* pow_s = reinterpret_cast<float*>(smem + T::OFF_POW);
+  float* pow_s = reinterpret_cast<float*>(smem + T::OFF_POW) + 32;  // pow_s[n] = lambda^n, 0 for n in [-32, -1]
   // barriers: raw tiles have landed / tiles are ready (k: weighted, by halves of 64 tokens) / tiles are free; scores ready,
   // decayed scores ready, chunk sum ready / read, state operand ready / read, outputs ready / read
   const uint32_t bar = sm + T::OFF_BAR;
-  const uint32_t kraw = bar, qraw = bar + 8, vraw = bar + 16, wfull = bar + 24 /* 2 */, qfull = bar + 40, vfull = bar + 48;
-  const uint32_t kempty = bar + 56, qempty = bar + 64, vempty = bar + 72, wempty = bar + 80 /* 2 */;
-  const uint32_t scready = bar + 96, dsready = bar + 104, sopread = bar + 112, oready = bar + 120;
-  const uint32_t pready = bar + 128, dsread = bar + 136, sopready = bar + 144, oread = bar + 152;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 160);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 164);
+  // (a pair is indexed by the half of the tokens or keys, or by the buffer, so that no wait can be two phases late)
+  const uint32_t kraw = bar, vraw = bar + 8 /* 2 */, qraw = bar + 24 /* 2 */, kempty = bar + 40, vempty = bar + 48 /* 2 */;
+  const uint32_t qempty = bar + 64 /* 2 */, wempty = bar + 80 /* 2 */, scready = bar + 96 /* 2 */, dsready = bar + 112;
+  const uint32_t sopread = bar + 120, oready = bar + 128;                                        // 17 of one arrival
+  const uint32_t wfull = bar + 136 /* 2 */, vfull = bar + 152, qfull = bar + 160;
+  const uint32_t pready = bar + 168 /* 2 */, rsready = bar + 184 /* 2 */, dsread = bar + 200, sopready = bar + 208, oread = bar + 216;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 240);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 244);
 
   const int h = blockIdx.x, seg = blockIdx.y, b = blockIdx.z;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
@@ -125,25 +158,21 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const int64_t per = (int64_t)(D + 1) * D;
 
   if (tid == 0) {
-    for (int i = 0; i < 20; ++i) mbar_init(bar + 8 * i, i >= 16 ? 4 : 1);
-    mbar_init(wfull, LW / 2);
-    mbar_init(wfull + 8, LW / 2);
-    mbar_init(qfull, LW);
-    mbar_init(vfull, LW);
+    for (int i = 0; i < 28; ++i) mbar_init(bar + 8 * i, i < 17 ? 1 : i < 19 ? LW / 2 : i < 21 ? LW : 4);
     if (!OUT) mbar_init(kempty, LW);  // no scores: k is free once it has been weighted
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 160), "r"((uint32_t)T::TMEM_COLS)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 240), "r"((uint32_t)T::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  for (int i = tid; i <= C; i += T::THREADS) pow_s[i] = ld_power(gl, i);
+  for (int i = tid - 32; i <= C; i += T::THREADS) pow_s[i] = i < 0 ? 0.f : ld_power(gl, i);
   // the ones column of v1 and its padding, once: token t, channels D .. D + 15 = two 16-byte pieces
-  for (int i = tid; i < 2 * C; i += T::THREADS) {
-    const int t = i >> 1, ch = D / 8 + (i & 1);
-    *reinterpret_cast<uint4*>(smem + T::OFF_V + (ch >> 3) * LT_BLK + t * 128 + (((ch & 7) ^ (t & 7)) << 4)) =
+  for (int i = tid; i < 2 * C * T::VBUF; i += T::THREADS) {
+    const int t = (i >> 1) % C, ch = D / 8 + (i & 1);
+    *reinterpret_cast<uint4*>(smem + T::OFF_V + i / (2 * C) * T::VTILE + (ch >> 3) * LT_BLK + t * 128 + (((ch & 7) ^ (t & 7)) << 4)) =
         make_uint4((i & 1) ? 0u : 0x3f80u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
@@ -161,13 +190,21 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const int j = tid;            // key channel (state)
     const int t = tid;            // query of the chunk (outputs)
     const bool jin = j < D, warp_in = warp * 32 < D;
-    float S[D + 1];
+    // Narrow heads: lane = key channel, warp w holds value channels 8 w .. + 7 and (warp 3) the key sum; else thread = key
+    // channel holds all of them.
+    constexpr int NS = T::STACK ? 9 : D + 1;
+    const int sj = T::STACK ? lane : j;
+    const bool sin = T::STACK ? lane < D : jin;
+    auto row_of = [&](int i) -> int { return !T::STACK ? i : i == 8 ? D : 8 * warp + i; };
+    auto held = [&](int i) -> bool { return !T::STACK || (i == 8 ? warp == 3 : 8 * warp < D); };
+    float S[NS];
 #pragma unroll
-    for (int i = 0; i <= D; ++i) S[i] = 0.f;
-    if (OUT && jin) {  // the state before this segment
+    for (int i = 0; i < NS; ++i) S[i] = 0.f;
+    if (OUT && sin) {  // the state before this segment
       auto add = [&](const float* src, float f) {
 #pragma unroll
-        for (int i = 0; i <= D; ++i) S[i] = fmaf(f, __ldg(src + i * D + j), S[i]);
+        for (int i = 0; i < NS; ++i)
+          if (held(i)) S[i] = fmaf(f, __ldg(src + row_of(i) * D + sj), S[i]);
       };
       if (a.prior) add(a.prior + ((int64_t)b * a.H + h) * per, ld_power(gl, n_begin));
       for (int r = 0; r < seg; ++r) {
@@ -180,12 +217,22 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const float* src = a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
         const float f = ld_power(gl, n_end - n_begin);
 #pragma unroll
-        for (int i = 0; i <= D; ++i) dst[i * D + j] = fmaf(f, S[i], n_end > n_begin ? __ldg(src + i * D + j) : 0.f);
+        for (int i = 0; i < NS; ++i)
+          if (held(i)) dst[row_of(i) * D + sj] = fmaf(f, S[i], n_end > n_begin ? __ldg(src + row_of(i) * D + sj) : 0.f);
       }
     }
-    // row j of the state operand: value channels 16 c .. + 15 as two 16-byte pieces
+    // row j of the state operand, 8 value channels to a 16-byte piece
     auto write_operand = [&]() {
-      if (jin) {
+      if constexpr (T::STACK) {
+        unsigned char* row = smem + T::OFF_S + lane * 128;
+        auto put = [&](int c, const uint4& w) { *reinterpret_cast<uint4*>(row + ((c ^ (lane & 7)) << 4)) = w; };  // c < 8
+        if (lane < D && 8 * warp < D)
+          put(warp, make_uint4(pack_bf16(S[0], S[1]), pack_bf16(S[2], S[3]), pack_bf16(S[4], S[5]), pack_bf16(S[6], S[7])));
+        if (lane < D && warp == 3) {
+          put(D / 8, make_uint4(pack_bf16(S[8], 0.f), 0u, 0u, 0u));
+          put(D / 8 + 1, make_uint4(0u, 0u, 0u, 0u));
+        }
+      } else if (jin) {
         unsigned char* row = smem + T::OFF_S + j * 128;
 #pragma unroll
         for (int c = 0; c < NV / 8; ++c) {
@@ -193,7 +240,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 8 * c + 2 * e;
-            w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? pack_bf16(S[D], 0.f) : 0u;
+            w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? pack_bf16(S[NS - 1], 0.f) : 0u;
           }
           *reinterpret_cast<uint4*>(row + (c >> 3) * T::STATE_BLK + (((c & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -207,74 +254,59 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int c = 0; c < chunks; ++c) {
       const uint32_t ph = (uint32_t)(c & 1);
       const int n0 = n_begin + c * C, nv = min(C, n_end - n0);
-      if (!mbar_wait(dsready, ph, abort_flag, 1, &g_ld_status)) { ok = false; break; }
+      if (!lt_wait(dsready, ph, abort_flag, 1)) { ok = false; break; }
       tcgen05_fence_after();
-      if constexpr (T::STACK) {  // warps 1 .. NT - 1 hold the sums of the lesser terms, lane = key channel
-        float* x = reinterpret_cast<float*>(smem + T::OFF_X);
-        if (warp > 0 && warp < NT) {
+      if constexpr (T::STACK) {  // warp s holds the sum of term s, lane = key channel: through shared memory, then warp by channels
+        float* x = reinterpret_cast<float*>(smem + T::OFF_X) + lane;
+        if (warp < NT) {
+          uint32_t d[NV];
 #pragma unroll
-          for (int g = 0; g < D / 16; ++g) {
-            uint32_t d[16];
-            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[((warp - 1) * (D + 1) + 16 * g + e) * 32 + lane] = __uint_as_float(d[e]);
-          }
-          const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
+          for (int g = 0; g < D / 16; ++g) tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), *reinterpret_cast<uint32_t(*)[16]>(d + 16 * g));
+          d[D] = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
           tmem_ld_wait();
-          x[((warp - 1) * (D + 1) + D) * 32 + lane] = __uint_as_float(d);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (warp == 0) {
-          const float whole = pow_s[nv];
-          auto join = [&](int i, uint32_t d) {
-            float r = x[i * 32 + lane];
-            if (NT == 3) r += x[(D + 1 + i) * 32 + lane];
-            S[i] = fmaf(whole, S[i], __uint_as_float(d) + r);
-          };
 #pragma unroll
-          for (int g = 0; g < D / 16; ++g) {
-            uint32_t d[16];
-            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) join(16 * g + e, d[e]);
-          }
-          const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
-          tmem_ld_wait();
-          join(D, d);
+          for (int i = 0; i <= D; ++i) x[(warp * (D + 1) + i) * 32] = __uint_as_float(d[i]);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the scratch is free again
-      } else if (warp_in) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the scratch is free again once every warp has arrived at dsread
         const float whole = pow_s[nv];
 #pragma unroll
-        for (int g = 0; g < D / 16; ++g) {
-          uint32_t d[16];
-          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), d);
-          tmem_ld_wait();
+        for (int i = 0; i < NS; ++i)
+          if (held(i)) {
+            float r = x[(D + 1 + row_of(i)) * 32];
+            if (NT == 3) r += x[(2 * (D + 1) + row_of(i)) * 32];
+            S[i] = fmaf(whole, S[i], x[row_of(i) * 32] + r);
+          }
+      } else if (warp_in) {
+        const float whole = pow_s[nv];
+        uint32_t d[2][16];  // the next columns are under way while these are added
+        tmem_ld_32x16(tmem + lanes + (uint32_t)T::COL_DS, d[0]);
+        const uint32_t z = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[16 * g + e] = fmaf(whole, S[16 * g + e], __uint_as_float(d[e]));
+        for (int g = 0; g < D / 16; ++g) {
+          tmem_ld_wait();
+          if (g + 1 < D / 16) tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * (g + 1)), d[(g + 1) & 1]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[16 * g + e] = fmaf(whole, S[16 * g + e], __uint_as_float(d[g & 1][e]));
         }
-        const uint32_t d = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
-        tmem_ld_wait();
-        S[D] = fmaf(whole, S[D], __uint_as_float(d));
+        S[NS - 1] = fmaf(whole, S[NS - 1], __uint_as_float(z));
       }
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dsread);
       if (OUT) {
         if (c + 1 < chunks) {
-          if (!mbar_wait(sopread, ph, abort_flag, 2, &g_ld_status)) { ok = false; break; }
+          if (!lt_wait(sopread, ph, abort_flag, 2)) { ok = false; break; }
           write_operand();
         }
-        if (!mbar_wait(oready, ph, abort_flag, 3, &g_ld_status)) { ok = false; break; }
+        if (!lt_wait(oready, ph, abort_flag, 3)) { ok = false; break; }
         tcgen05_fence_after();
         const float f = pow_s[t + 1];
         float m = a.scale;
         if (a.normalise) {
-          const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D)), d2 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O2 + D));
+          if (!lt_wait(rsready + 8 * ph, (uint32_t)(c >> 1) & 1u, abort_flag, 3)) { ok = false; break; }
+          const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D));
           tmem_ld_wait();
-          m = 1.f / (fmaf(f, __uint_as_float(d1), __uint_as_float(d2)) + a.eps);
+          m = 1.f / (fmaf(f, __uint_as_float(d1), reinterpret_cast<const float*>(smem + T::OFF_RS)[(c & 1) * C + t]) + a.eps);
         }
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row0 + n0 + t) * a.ldo + (int64_t)h * D;
 #pragma unroll
@@ -297,10 +329,11 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (lane == 0) mbar_arrive(oread);
       }
     }
-    if (ok && jin && (!OUT || (a.npart == 0 && seg == a.nseg - 1))) {
+    if (ok && sin && (!OUT || (a.npart == 0 && seg == a.nseg - 1))) {
       float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
 #pragma unroll
-      for (int i = 0; i <= D; ++i) dst[i * D + j] = S[i];
+      for (int i = 0; i < NS; ++i)
+        if (held(i)) dst[row_of(i) * D + sj] = S[i];
     }
   } else if (warp < 8) {
     // ------------------------------- scores --------------------------------------------
@@ -308,40 +341,57 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (OUT) {
       const int w = warp - 4;
       const uint32_t sc = tmem + ((uint32_t)(w * 32) << 16) + (uint32_t)T::COL_SC;
+      float* rs = reinterpret_cast<float*>(smem + T::OFF_RS) + 32 * w + lane;
+      const float* mine = pow_s + lane;
       for (int c = 0; c < chunks; ++c) {
-        if (!mbar_wait(scready, (uint32_t)(c & 1), abort_flag, 4, &g_ld_status)) break;
-        tcgen05_fence_after();
+        float sum = 0.f;
+        bool ok = true;
 #pragma unroll 1
-        for (int blk = 0; blk < 4; ++blk) {  // keys 32 blk .. + 31; the bf16 pairs go over scores that have been read
-          uint32_t p[16];
-          if (blk > w) {
+        for (int half = 0; half < 2; ++half) {  // rolled: four roles share the instruction cache
+          if (!lt_wait(scready + 8 * half, (uint32_t)(c & 1), abort_flag, 4)) { ok = false; break; }
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {  // keys 32 blk .. + 31; the bf16 pairs go over scores that have been read
+            const int blk = 2 * half + q;
+            uint32_t p[16];
+            if (blk > w) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = 0u;
-          } else {
-            uint32_t x[32];
-            tmem_ld_32x32(sc + (uint32_t)(32 * blk), x);
-            tmem_ld_wait();
-            if (blk < w) {  // every key lies before every query: lambda^(t - s) = lambda^(t - s0 - 31) lambda^(31 - k)
-              const float f = pow_s[32 * (w - blk) + lane - 31];
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                p[e] = pack_bf16(__uint_as_float(x[2 * e]) * (f * pow_s[31 - 2 * e]), __uint_as_float(x[2 * e + 1]) * (f * pow_s[30 - 2 * e]));
+              for (int e = 0; e < 16; ++e) p[e] = 0u;
             } else {
+              uint32_t x[32];
+              tmem_ld_32x32(sc + (uint32_t)(32 * blk), x);
+              tmem_ld_wait();
+              if (blk < w) {  // every key lies before every query: lambda^(t - s) = lambda^(t - s0 - 31) lambda^(31 - k)
+                const float f = mine[32 * (w - blk) - 31];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int d0 = lane - 2 * e, d1 = d0 - 1;  // t - s
-                const float p0 = d0 >= 0 ? __uint_as_float(x[2 * e]) * pow_s[max(d0, 0)] : 0.f;
-                const float p1 = d1 >= 0 ? __uint_as_float(x[2 * e + 1]) * pow_s[max(d1, 0)] : 0.f;
-                p[e] = pack_bf16(p0, p1);
+                for (int e = 0; e < 16; ++e) {
+                  const float p0 = __uint_as_float(x[2 * e]) * (f * pow_s[31 - 2 * e]);
+                  const float p1 = __uint_as_float(x[2 * e + 1]) * (f * pow_s[30 - 2 * e]);
+                  sum += p0 + p1;
+                  p[e] = pack_bf16(p0, p1);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {  // selected, not multiplied by the table's zero: a later token may be NaN
+                  const float p0 = lane >= 2 * e ? __uint_as_float(x[2 * e]) * mine[-2 * e] : 0.f;
+                  const float p1 = lane >= 2 * e + 1 ? __uint_as_float(x[2 * e + 1]) * mine[-2 * e - 1] : 0.f;
+                  sum += p0 + p1;
+                  p[e] = pack_bf16(p0, p1);
+                }
               }
             }
+            lt_st16(sc + (uint32_t)(64 * half + 16 * q), p);
           }
-          lt_st16(sc + (uint32_t)(16 * blk), p);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          if (half == 1 && a.normalise) rs[(c & 1) * C] = sum;
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(pready + 8 * half);
+            if (half == 1 && a.normalise) mbar_arrive(rsready + 8 * (c & 1));
+          }
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pready);
+        if (!ok) break;
       }
       // rows of the segment past the sequence are zeros
       const int z0 = max(seg_begin, n_end);
@@ -372,8 +422,8 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const uint32_t ph = (uint32_t)(c & 1);
       const int nv = min(C, n_end - (n_begin + c * C));
       const bool live = row < nv;
-      if (!mbar_wait(kraw, ph, abort_flag, 5, &g_ld_status)) break;
-      if (!mbar_wait(wempty + wbar, ph ^ 1u, abort_flag, 6, &g_ld_status)) break;
+      if (!lt_wait(kraw, ph, abort_flag, 5)) break;
+      if (!lt_wait(wempty + wbar, ph ^ 1u, abort_flag, 6)) break;
       const float wt = live ? pow_s[nv - 1 - row] : 0.f;
 #pragma unroll
       for (int i = 0; i < D / 8 / PARTS; ++i) {
@@ -401,22 +451,23 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (!OUT) {
         if (lane == 0) mbar_arrive(kempty);
       } else {
-        if (!mbar_wait(qraw, ph, abort_flag, 7, &g_ld_status)) break;
+        if (!lt_wait(qraw + 8 * (c % T::QBUF), (uint32_t)(c / T::QBUF) & 1u, abort_flag, 7)) break;
         if (relu) {
 #pragma unroll
           for (int i = 0; i < D / 8 / PARTS; ++i) {
-            uint4* p = reinterpret_cast<uint4*>(qrow + piece(i * PARTS + part));
+            uint4* p = reinterpret_cast<uint4*>(qrow + c % T::QBUF * T::KTILE + piece(i * PARTS + part));
             *p = relu4(*p);
           }
         }
         publish(qfull);
       }
-      if (!mbar_wait(vraw, ph, abort_flag, 8, &g_ld_status)) break;
+      unsigned char* vt = vrow + c % T::VBUF * T::VTILE;
+      if (!lt_wait(vraw + 8 * (c % T::VBUF), (uint32_t)(c / T::VBUF) & 1u, abort_flag, 8)) break;
       if (!live) {  // rows behind the sequence meet zero weights: they must be finite
 #pragma unroll
-        for (int i = 0; i < D / 8 / PARTS; ++i) *reinterpret_cast<uint4*>(vrow + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < D / 8 / PARTS; ++i) *reinterpret_cast<uint4*>(vt + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
       }
-      if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vrow + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
+      if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vt + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
       publish(vfull);
     }
   } else {
@@ -424,35 +475,42 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if constexpr (T::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 8 + LW) {  // the whole warp waits, one elected lane issues
       const uint32_t Wu = sm + T::OFF_W, Vu = sm + T::OFF_V, Ku = sm + T::OFF_K, Qu = sm + T::OFF_Q, Su = sm + T::OFF_S;
-      const uint64_t vdesc = lt_desc_mn(Vu, LT_BLK), sdesc = lt_desc_mn(Su, T::STATE_BLK);
+      const uint64_t sdesc = lt_desc_mn(Su, T::STATE_BLK);
       auto wait = [&](uint32_t bb, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(bb, parity, abort_flag, code, &g_ld_status));
+        return __all_sync(0xffffffffu, lt_wait(bb, parity, abort_flag, code));
       };
-      for (int c = 0; c < chunks; ++c) {
+      auto qtile = [&](int c) -> uint32_t { return Qu + (uint32_t)(c % T::QBUF * T::KTILE); };
+      auto scores = [&](int c, int half) -> bool {  // keys 64 half .. + 63 of chunk c
         const uint32_t ph = (uint32_t)(c & 1);
-        if (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10)) break;
-        if (OUT) {
-          if (!wait(qfull, ph, 11) || !wait(oread, ph ^ 1u, 12)) break;  // the previous outputs lie over the scores
-          tcgen05_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_bf16(tmem + T::COL_SC, make_smem_desc(Qu + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)),
-                        make_smem_desc(Ku + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), T::ID_SC, k != 0 ? 1u : 0u);
-            umma_commit(scready);
-            umma_commit(kempty);
-          }
-          __syncwarp();
+        if (!wait(wfull + 8 * half, ph, 10)) return false;
+        if (half == 0 && !wait(qfull, ph, 11)) return false;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          const uint32_t Qc = qtile(c);
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + T::COL_SC + 64 * half, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)),
+                      make_smem_desc(Ku + half * 8192 + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), T::ID_SC, k != 0 ? 1u : 0u);
+          umma_commit(scready + 8 * half);
+          if (half == 1) umma_commit(kempty);
         }
+        __syncwarp();
+        return true;
+      };
+      bool ok = !OUT || chunks == 0 || (scores(0, 0) && scores(0, 1));
+      for (int c = 0; c < chunks && ok; ++c) {
+        const uint32_t ph = (uint32_t)(c & 1);
+        const uint64_t vdesc = lt_desc_mn(Vu + (uint32_t)(c % T::VBUF * T::VTILE), LT_BLK);
+        if (!OUT && (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10))) break;
         if (!wait(vfull, ph, 13) || !wait(dsread, ph ^ 1u, 14)) break;
         tcgen05_fence_after();
         if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-#pragma unroll
+#pragma unroll 1
             for (int s = T::MMAS - 1; s >= 0; --s) {  // smallest term first
               const uint64_t wdesc = lt_desc_mn(Wu + s * T::KTILE, LT_BLK);
-#pragma unroll
+#pragma unroll 1
               for (int k = 4 * half; k < 4 * half + 4; ++k)
                 umma_bf16(tmem + T::COL_DS, wdesc + (uint64_t)(128 * k), vdesc + (uint64_t)(128 * k), T::ID_DS,
                           (half != 0 || s != T::MMAS - 1 || k != 0) ? 1u : 0u);
@@ -460,31 +518,43 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             umma_commit(wempty + 8 * half);
           }
           umma_commit(dsready);
-          if (!OUT) umma_commit(vempty);
+          if (!OUT) umma_commit(vempty + 8 * (c % T::VBUF));
         }
         __syncwarp();
         if (!OUT) continue;
-        if (!wait(sopready, ph, 15)) break;
+        if (!wait(sopready, ph, 15) || !wait(oread, ph ^ 1u, 12)) break;
         tcgen05_fence_after();
         if (elect_one()) {
-#pragma unroll
+          const uint32_t Qc = qtile(c);
+#pragma unroll 1
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qu + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
-                      T::ID_O, k != 0 ? 1u : 0u);
-          umma_commit(qempty);
+            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
+                      T::ID_O1, k != 0 ? 1u : 0u);
+          umma_commit(qempty + 8 * (c % T::QBUF));
           umma_commit(sopread);
         }
         __syncwarp();
-        if (!wait(pready, ph, 16)) break;
-        tcgen05_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < C / 16; ++k)
-            lt_mma_ts(tmem + T::COL_O2, tmem + T::COL_SC + 8u * k, vdesc + (uint64_t)(128 * k), T::ID_O, k != 0 ? 1u : 0u);
-          umma_commit(vempty);
-          umma_commit(oready);
+        // the decayed scores of a half meet v, then the next chunk's scores take their columns (products run in order)
+#pragma unroll 1
+        for (int half = 0; half < 2 && ok; ++half) {
+          if (!wait(pready + 8 * half, ph, 16)) { ok = false; break; }
+          tcgen05_fence_after();
+          if (!T::ALIAS || half == 1) {
+            if (elect_one()) {
+#pragma unroll 1
+              for (int k = T::ALIAS ? 0 : 4 * half; k < 4 * half + 4; ++k)
+                lt_mma_ts(tmem + T::COL_O2, tmem + T::COL_SC + 64u * (k >> 2) + 8u * (k & 3), vdesc + (uint64_t)(128 * k), T::ID_O2,
+                          k != 0 ? 1u : 0u);
+              if (half == 1) {
+                umma_commit(vempty + 8 * (c % T::VBUF));
+                umma_commit(oready);
+              }
+            }
+            __syncwarp();
+          }
+          if (!T::ALIAS && c + 1 < chunks) ok = scores(c + 1, half);
         }
-        __syncwarp();
+        if (T::ALIAS && ok && c + 1 < chunks) ok = wait(oread, ph, 12) && scores(c + 1, 0) && scores(c + 1, 1);
       }
     } else if (warp == 9 + LW && lane == 0) {  // copies
       const int hk = h / a.group;
@@ -500,14 +570,16 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int c = 0; c < chunks; ++c) {
         const uint32_t ph = (uint32_t)(c & 1);
         const int n0 = n_begin + c * C;
-        if (!mbar_wait(kempty, ph ^ 1u, abort_flag, 17, &g_ld_status)) break;
+        if (!lt_wait(kempty, ph ^ 1u, abort_flag, 17)) break;
         copy(sm + T::OFF_K, &tmK, kraw, hk, n0);
         if (OUT) {
-          if (!mbar_wait(qempty, ph ^ 1u, abort_flag, 18, &g_ld_status)) break;
-          copy(sm + T::OFF_Q, &tmQ, qraw, h, n0);
+          const int qb = c % T::QBUF;
+          if (!lt_wait(qempty + 8 * qb, ((uint32_t)(c / T::QBUF) & 1u) ^ 1u, abort_flag, 18)) break;
+          copy(sm + T::OFF_Q + (uint32_t)(qb * T::KTILE), &tmQ, qraw + 8 * qb, h, n0);
         }
-        if (!mbar_wait(vempty, ph ^ 1u, abort_flag, 19, &g_ld_status)) break;
-        copy(sm + T::OFF_V, &tmV, vraw, hk, n0);
+        const int vb = c % T::VBUF;
+        if (!lt_wait(vempty + 8 * vb, ((uint32_t)(c / T::VBUF) & 1u) ^ 1u, abort_flag, 19)) break;
+        copy(sm + T::OFF_V + (uint32_t)(vb * T::VTILE), &tmV, vraw + 8 * vb, hk, n0);
       }
     }
   }
