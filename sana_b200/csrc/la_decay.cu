@@ -745,7 +745,7 @@ extern "C" int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t 
   SANA_REQUIRE(prior != state, "sana_la_decay: prior and state must be different buffers");
   SANA_REQUIRE(workspace || workspace_bytes == 0, "sana_la_decay: null workspace");
   LdArgs a = {q, k, v, ldq, ldk, ldv, log_decay, prior, lengths, static_cast<float*>(workspace), state, out, ldo, (int)N, (int)H,
-              (int)(H / Hk), 0, 0, 0, scale, eps, relu ? 1 : 0, eps >= 0.f ? 1 : 0};
+              (int)(H / Hk), 0, 0, 0, scale, eps, relu ? 1 : 0, eps >= 0.f ? 1 : 0, 0};
   LD_DISPATCH(D, return (launch_decay<HD>(a, B, dtype, workspace_bytes, static_cast<cudaStream_t>(stream))));
   return SANA_ERR_INVALID;
 }

@@ -19,6 +19,7 @@ struct LdArgs {
   int seg_len, nseg, npart;
   float scale, eps;
   int relu, normalise;
+  int wide_rows;             // output rows are 32-byte aligned
 };
 
 __device__ __forceinline__ float ld_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }

@@ -309,20 +309,31 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           m = 1.f / (fmaf(f, __uint_as_float(d1), reinterpret_cast<const float*>(smem + T::OFF_RS)[(c & 1) * C + t]) + a.eps);
         }
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row0 + n0 + t) * a.ldo + (int64_t)h * D;
-#pragma unroll
+        uint32_t x[16], y[16];
+        tmem_ld_32x16(tmem + lanes + (uint32_t)T::COL_O1, x);
+        tmem_ld_32x16(tmem + lanes + (uint32_t)T::COL_O2, y);
+        tmem_ld_wait();
+#pragma unroll 1
         for (int g = 0; g < D / 16; ++g) {
-          uint32_t x[16], y[16], w[8];
-          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O1 + 16 * g), x);
-          tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O2 + 16 * g), y);
-          tmem_ld_wait();
+          uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             w[e] = pack_bf16(fmaf(f, __uint_as_float(x[2 * e]), __uint_as_float(y[2 * e])) * m,
                              fmaf(f, __uint_as_float(x[2 * e + 1]), __uint_as_float(y[2 * e + 1])) * m);
-          if (t < nv) {
-            *reinterpret_cast<uint4*>(dst + 16 * g) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(dst + 16 * g + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          if (g + 1 < D / 16) {  // the next columns are under way while these are stored
+            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O1 + 16 * (g + 1)), x);
+            tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O2 + 16 * (g + 1)), y);
           }
+          if (t < nv) {
+            if (a.wide_rows) {  // 32-byte aligned rows: whole sectors
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * g), "r"(w[0]), "r"(w[1]),
+                           "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+            } else {
+              *reinterpret_cast<uint4*>(dst + 16 * g) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(dst + 16 * g + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+          }
+          tmem_ld_wait();
         }
         tcgen05_fence_before();
         __syncwarp();
@@ -425,26 +436,35 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (!lt_wait(kraw, ph, abort_flag, 5)) break;
       if (!lt_wait(wempty + wbar, ph ^ 1u, abort_flag, 6)) break;
       const float wt = live ? pow_s[nv - 1 - row] : 0.f;
+      constexpr int PIECES = D / 8 / PARTS, STEP = PIECES % 2 == 0 ? 2 : PIECES == 7 ? 7 : 5;
+      static_assert(PIECES % STEP == 0, "whole steps");
+#pragma unroll 1
+      for (int i0 = 0; i0 < PIECES; i0 += STEP) {  // rolled, as is every loop here that may be: the roles share the instruction cache
+        uint4 r[STEP];
 #pragma unroll
-      for (int i = 0; i < D / 8 / PARTS; ++i) {
-        const int ch = i * PARTS + part;
-        uint4* kp = reinterpret_cast<uint4*>(krow + piece(ch));
-        uint4 r = *kp;
-        if (relu) {
-          r = relu4(r);
-          if (OUT) *kp = r;
-        }
-        if (!live) r = make_uint4(0u, 0u, 0u, 0u);  // whatever lies behind the sequence
-        uint32_t w[4] = {r.x, r.y, r.z, r.w};
-        float x[4], y[4];
+        for (int i = 0; i < STEP; ++i) r[i] = *reinterpret_cast<const uint4*>(krow + piece((i0 + i) * PARTS + part));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = bf16_lo(w[e]) * wt, y[e] = bf16_hi(w[e]) * wt;
+        for (int i = 0; i < STEP; ++i) {
+          const int ch = (i0 + i) * PARTS + part;
+          if (relu) {
+            r[i] = relu4(r[i]);
+            if (OUT) *reinterpret_cast<uint4*>(krow + piece(ch)) = r[i];
+          }
+          if (!live) r[i] = make_uint4(0u, 0u, 0u, 0u);  // whatever lies behind the sequence
+          uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+          float2 x[4];
 #pragma unroll
-        for (int s = 0; s < NT; ++s) {
+          for (int e = 0; e < 4; ++e) x[e] = __fmul2_rn(make_float2(bf16_lo(w[e]), bf16_hi(w[e])), make_float2(wt, wt));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = s + 1 < NT ? ld_split(x[e], y[e]) : pack_bf16(x[e], y[e]);
-          const uint32_t at = T::STACK ? piece(ch + 4 * s) : (uint32_t)(s * T::KTILE) + piece(ch);
-          *reinterpret_cast<uint4*>(smem + T::OFF_W + row * 128 + at) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int s = 0; s < NT; ++s) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[e] = pack_bf16(x[e].x, x[e].y);
+              if (s + 1 < NT) x[e] = __fadd2_rn(x[e], make_float2(-bf16_lo(w[e]), -bf16_hi(w[e])));
+            }
+            const uint32_t at = T::STACK ? piece(ch + 4 * s) : (uint32_t)(s * T::KTILE) + piece(ch);
+            *reinterpret_cast<uint4*>(smem + T::OFF_W + row * 128 + at) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
       }
       publish(wfull + wbar);
@@ -453,19 +473,20 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       } else {
         if (!lt_wait(qraw + 8 * (c % T::QBUF), (uint32_t)(c / T::QBUF) & 1u, abort_flag, 7)) break;
         if (relu) {
+          unsigned char* qt = qrow + c % T::QBUF * T::KTILE;
+          uint4 r[PIECES];
 #pragma unroll
-          for (int i = 0; i < D / 8 / PARTS; ++i) {
-            uint4* p = reinterpret_cast<uint4*>(qrow + c % T::QBUF * T::KTILE + piece(i * PARTS + part));
-            *p = relu4(*p);
-          }
+          for (int i = 0; i < PIECES; ++i) r[i] = *reinterpret_cast<const uint4*>(qt + piece(i * PARTS + part));
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4*>(qt + piece(i * PARTS + part)) = relu4(r[i]);
         }
         publish(qfull);
       }
       unsigned char* vt = vrow + c % T::VBUF * T::VTILE;
       if (!lt_wait(vraw + 8 * (c % T::VBUF), (uint32_t)(c / T::VBUF) & 1u, abort_flag, 8)) break;
       if (!live) {  // rows behind the sequence meet zero weights: they must be finite
-#pragma unroll
-        for (int i = 0; i < D / 8 / PARTS; ++i) *reinterpret_cast<uint4*>(vt + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4*>(vt + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
       }
       if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vt + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
       publish(vfull);
@@ -502,6 +523,20 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const uint32_t ph = (uint32_t)(c & 1);
         const uint64_t vdesc = lt_desc_mn(Vu + (uint32_t)(c % T::VBUF * T::VTILE), LT_BLK);
         if (!OUT && (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10))) break;
+        if (OUT) {
+        if (!wait(sopready, ph, 15) || !wait(oread, ph ^ 1u, 12)) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          const uint32_t Qc = qtile(c);
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
+                      T::ID_O1, k != 0 ? 1u : 0u);
+          umma_commit(qempty + 8 * (c % T::QBUF));
+          umma_commit(sopread);
+        }
+        __syncwarp();
+        }
         if (!wait(vfull, ph, 13) || !wait(dsread, ph ^ 1u, 14)) break;
         tcgen05_fence_after();
         if (elect_one()) {
@@ -522,18 +557,6 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         __syncwarp();
         if (!OUT) continue;
-        if (!wait(sopready, ph, 15) || !wait(oread, ph ^ 1u, 12)) break;
-        tcgen05_fence_after();
-        if (elect_one()) {
-          const uint32_t Qc = qtile(c);
-#pragma unroll 1
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
-                      T::ID_O1, k != 0 ? 1u : 0u);
-          umma_commit(qempty + 8 * (c % T::QBUF));
-          umma_commit(sopread);
-        }
-        __syncwarp();
         // the decayed scores of a half meet v, then the next chunk's scores take their columns (products run in order)
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half) {
@@ -567,9 +590,22 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
               ::"r"(dst + i * LT_BLK), "l"(tm), "r"(full), "r"(64 * i), "r"(head), "r"(n0), "r"(b)
               : "memory");
       };
+      // a tile is free only shortly before it is needed again: what it will take is brought into L2 two chunks ahead
+      auto prefetch = [&](const CUtensorMap* tm, int head, int n0) {
+#pragma unroll
+        for (int i = 0; i < T::KB; ++i)
+          asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(tm), "r"(64 * i), "r"(head), "r"(n0), "r"(b)
+                       : "memory");
+      };
       for (int c = 0; c < chunks; ++c) {
         const uint32_t ph = (uint32_t)(c & 1);
         const int n0 = n_begin + c * C;
+        for (int ahead = c == 0 ? 1 : 2; ahead <= 2; ++ahead)
+          if (c + ahead < chunks) {
+            prefetch(&tmK, hk, n0 + ahead * C);
+            if (OUT) prefetch(&tmQ, h, n0 + ahead * C);
+            prefetch(&tmV, hk, n0 + ahead * C);
+          }
         if (!lt_wait(kempty, ph ^ 1u, abort_flag, 17)) break;
         copy(sm + T::OFF_K, &tmK, kraw, hk, n0);
         if (OUT) {
@@ -656,6 +692,7 @@ LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, int* npart) {
 }
 
 int launch_decay_tc(LdArgs& a, int64_t B, int64_t D, cudaStream_t st) {
+  a.wide_rows = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && a.ldo % 16 == 0;
   switch (D) {
     case 16: return lt_run<16>(a, B, st);
     case 32: return lt_run<32>(a, B, st);
