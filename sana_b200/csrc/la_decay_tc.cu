@@ -42,7 +42,7 @@ struct Lt {
   static constexpr int KTILE = KB * LT_BLK, VTILE = VB * LT_BLK;
   static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
   static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
-  static constexpr int X_BYTES = STACK ? NT * (D + 1) * 32 * 4 : 0;  // sums of the terms, [NT][D+1][32]
+  static constexpr int X_BYTES = STACK ? (D + 1) * 32 * (NT == 3 ? 10 : 8) : 0;  // sums of the terms, [D+1][32]; the third in bf16
   static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 4) + (OUT ? 4 * 2 * LT_C : 0) + 8 * 32;
   static constexpr int ONE_EACH = WTILE + VTILE + KTILE + (OUT ? KTILE : 0) + SCRATCH;
   static constexpr int LIMIT = OUT && D <= 32 ? 113 * 1024 : 232448;  // two CTAs per SM, or one
@@ -136,15 +136,15 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     return;
   }
   float* pow_s = reinterpret_cast<float*>(smem + T::OFF_POW) + 32;  // pow_s[n] = lambda^n, 0 for n in [-32, -1]
-  // barriers: raw tiles have landed / tiles are ready (k: weighted, by halves of 64 tokens) / tiles are free; scores ready,
+  // barriers: raw tiles have landed / tiles are ready (weighted k: by halves of 64 tokens) / tiles are free; scores ready,
   // decayed scores ready, chunk sum ready / read, state operand ready / read, outputs ready / read
   const uint32_t bar = sm + T::OFF_BAR;
   // (a pair is indexed by the half of the tokens or keys, or by the buffer, so that no wait can be two phases late)
   const uint32_t kraw = bar, vraw = bar + 8 /* 2 */, qraw = bar + 24 /* 2 */, kempty = bar + 40, vempty = bar + 48 /* 2 */;
   const uint32_t qempty = bar + 64 /* 2 */, wempty = bar + 80 /* 2 */, scready = bar + 96 /* 2 */, dsready = bar + 112;
   const uint32_t sopread = bar + 120, oready = bar + 128;                                        // 17 of one arrival
-  const uint32_t wfull = bar + 136 /* 2 */, vfull = bar + 152, qfull = bar + 160;
-  const uint32_t pready = bar + 168 /* 2 */, rsready = bar + 184 /* 2 */, dsread = bar + 200, sopready = bar + 208, oread = bar + 216;
+  const uint32_t wfull = bar + 136 /* 2 */, vfull = bar + 152, qfull = bar + 160, kfull = bar + 168;
+  const uint32_t pready = bar + 176 /* 2 */, rsready = bar + 192 /* 2 */, dsread = bar + 208, sopready = bar + 216, oread = bar + 224;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 240);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 244);
 
@@ -158,7 +158,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const int64_t per = (int64_t)(D + 1) * D;
 
   if (tid == 0) {
-    for (int i = 0; i < 28; ++i) mbar_init(bar + 8 * i, i < 17 ? 1 : i < 19 ? LW / 2 : i < 21 ? LW : 4);
+    for (int i = 0; i < 29; ++i) mbar_init(bar + 8 * i, i < 17 ? 1 : i < 19 ? LW / 2 : i < 22 ? LW : 4);
     if (!OUT) mbar_init(kempty, LW);  // no scores: k is free once it has been weighted
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -258,6 +258,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       tcgen05_fence_after();
       if constexpr (T::STACK) {  // warp s holds the sum of term s, lane = key channel: through shared memory, then warp by channels
         float* x = reinterpret_cast<float*>(smem + T::OFF_X) + lane;
+        __nv_bfloat16* x3 = reinterpret_cast<__nv_bfloat16*>(smem + T::OFF_X + 2 * (D + 1) * 32 * 4) + lane;
         if (warp < NT) {
           uint32_t d[NV];
 #pragma unroll
@@ -265,7 +266,10 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           d[D] = lt_ld1(tmem + lanes + (uint32_t)(T::COL_DS + D));
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i <= D; ++i) x[(warp * (D + 1) + i) * 32] = __uint_as_float(d[i]);
+          for (int i = 0; i <= D; ++i) {
+            if (warp < 2) x[(warp * (D + 1) + i) * 32] = __uint_as_float(d[i]);
+            else x3[i * 32] = __float2bfloat16_rn(__uint_as_float(d[i]));  // 2^-16 of the first: its rounding is below 2^-24
+          }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the scratch is free again once every warp has arrived at dsread
         const float whole = pow_s[nv];
@@ -273,7 +277,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int i = 0; i < NS; ++i)
           if (held(i)) {
             float r = x[(D + 1 + row_of(i)) * 32];
-            if (NT == 3) r += x[(2 * (D + 1) + row_of(i)) * 32];
+            if (NT == 3) r += __bfloat162float(x3[row_of(i) * 32]);
             S[i] = fmaf(whole, S[i], x[row_of(i) * 32] + r);
           }
       } else if (warp_in) {
@@ -433,55 +437,55 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const uint32_t ph = (uint32_t)(c & 1);
       const int nv = min(C, n_end - (n_begin + c * C));
       const bool live = row < nv;
+      constexpr int PIECES = D / 8 / PARTS;
+      // features first: the next scores need them, the weights only when the state's products of the chunk before are done
       if (!lt_wait(kraw, ph, abort_flag, 5)) break;
-      if (!lt_wait(wempty + wbar, ph ^ 1u, abort_flag, 6)) break;
-      const float wt = live ? pow_s[nv - 1 - row] : 0.f;
-      constexpr int PIECES = D / 8 / PARTS, STEP = PIECES % 2 == 0 ? 2 : PIECES == 7 ? 7 : 5;
-      static_assert(PIECES % STEP == 0, "whole steps");
-#pragma unroll 1
-      for (int i0 = 0; i0 < PIECES; i0 += STEP) {  // rolled, as is every loop here that may be: the roles share the instruction cache
-        uint4 r[STEP];
+      uint4 r[PIECES];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) r[i] = *reinterpret_cast<const uint4*>(krow + piece((i0 + i) * PARTS + part));
-#pragma unroll
-        for (int i = 0; i < STEP; ++i) {
-          const int ch = (i0 + i) * PARTS + part;
-          if (relu) {
-            r[i] = relu4(r[i]);
-            if (OUT) *reinterpret_cast<uint4*>(krow + piece(ch)) = r[i];
-          }
-          if (!live) r[i] = make_uint4(0u, 0u, 0u, 0u);  // whatever lies behind the sequence
-          uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-          float2 x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = __fmul2_rn(make_float2(bf16_lo(w[e]), bf16_hi(w[e])), make_float2(wt, wt));
-#pragma unroll
-          for (int s = 0; s < NT; ++s) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[e] = pack_bf16(x[e].x, x[e].y);
-              if (s + 1 < NT) x[e] = __fadd2_rn(x[e], make_float2(-bf16_lo(w[e]), -bf16_hi(w[e])));
-            }
-            const uint32_t at = T::STACK ? piece(ch + 4 * s) : (uint32_t)(s * T::KTILE) + piece(ch);
-            *reinterpret_cast<uint4*>(smem + T::OFF_W + row * 128 + at) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+      for (int i = 0; i < PIECES; ++i) {
+        r[i] = *reinterpret_cast<const uint4*>(krow + piece(i * PARTS + part));
+        if (relu) {
+          r[i] = relu4(r[i]);
+          if (OUT) *reinterpret_cast<uint4*>(krow + piece(i * PARTS + part)) = r[i];
         }
       }
-      publish(wfull + wbar);
-      if (!OUT) {
-        if (lane == 0) mbar_arrive(kempty);
-      } else {
+      if constexpr (OUT) {
+        publish(kfull);
         if (!lt_wait(qraw + 8 * (c % T::QBUF), (uint32_t)(c / T::QBUF) & 1u, abort_flag, 7)) break;
         if (relu) {
           unsigned char* qt = qrow + c % T::QBUF * T::KTILE;
-          uint4 r[PIECES];
 #pragma unroll
-          for (int i = 0; i < PIECES; ++i) r[i] = *reinterpret_cast<const uint4*>(qt + piece(i * PARTS + part));
-#pragma unroll
-          for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4*>(qt + piece(i * PARTS + part)) = relu4(r[i]);
+          for (int i = 0; i < PIECES; ++i) {
+            uint4* p = reinterpret_cast<uint4*>(qt + piece(i * PARTS + part));
+            *p = relu4(*p);
+          }
         }
         publish(qfull);
+      } else {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kempty);
       }
+      if (!lt_wait(wempty + wbar, ph ^ 1u, abort_flag, 6)) break;
+      const float wt = live ? pow_s[nv - 1 - row] : 0.f;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int ch = i * PARTS + part;
+        uint32_t w[4] = {live ? r[i].x : 0u, live ? r[i].y : 0u, live ? r[i].z : 0u, live ? r[i].w : 0u};  // rows behind the sequence
+        float2 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __fmul2_rn(make_float2(bf16_lo(w[e]), bf16_hi(w[e])), make_float2(wt, wt));
+#pragma unroll
+        for (int s = 0; s < NT; ++s) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = pack_bf16(x[e].x, x[e].y);
+            if (s + 1 < NT) x[e] = __fadd2_rn(x[e], make_float2(-bf16_lo(w[e]), -bf16_hi(w[e])));
+          }
+          const uint32_t at = T::STACK ? piece(ch + 4 * s) : (uint32_t)(s * T::KTILE) + piece(ch);
+          *reinterpret_cast<uint4*>(smem + T::OFF_W + row * 128 + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      publish(wfull + wbar);
       unsigned char* vt = vrow + c % T::VBUF * T::VTILE;
       if (!lt_wait(vraw + 8 * (c % T::VBUF), (uint32_t)(c / T::VBUF) & 1u, abort_flag, 8)) break;
       if (!live) {  // rows behind the sequence meet zero weights: they must be finite
@@ -503,8 +507,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       auto qtile = [&](int c) -> uint32_t { return Qu + (uint32_t)(c % T::QBUF * T::KTILE); };
       auto scores = [&](int c, int half) -> bool {  // keys 64 half .. + 63 of chunk c
         const uint32_t ph = (uint32_t)(c & 1);
-        if (!wait(wfull + 8 * half, ph, 10)) return false;
-        if (half == 0 && !wait(qfull, ph, 11)) return false;
+        if (half == 0 && (!wait(kfull, ph, 17) || !wait(qfull, ph, 11))) return false;
         tcgen05_fence_after();
         if (elect_one()) {
           const uint32_t Qc = qtile(c);
@@ -522,22 +525,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int c = 0; c < chunks && ok; ++c) {
         const uint32_t ph = (uint32_t)(c & 1);
         const uint64_t vdesc = lt_desc_mn(Vu + (uint32_t)(c % T::VBUF * T::VTILE), LT_BLK);
-        if (!OUT && (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10))) break;
-        if (OUT) {
-        if (!wait(sopready, ph, 15) || !wait(oread, ph ^ 1u, 12)) break;
-        tcgen05_fence_after();
-        if (elect_one()) {
-          const uint32_t Qc = qtile(c);
-#pragma unroll 1
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
-                      T::ID_O1, k != 0 ? 1u : 0u);
-          umma_commit(qempty + 8 * (c % T::QBUF));
-          umma_commit(sopread);
-        }
-        __syncwarp();
-        }
-        if (!wait(vfull, ph, 13) || !wait(dsread, ph ^ 1u, 14)) break;
+        if (!wait(wfull, ph, 10) || !wait(wfull + 8, ph, 10) || !wait(vfull, ph, 13) || !wait(dsread, ph ^ 1u, 14)) break;
         tcgen05_fence_after();
         if (elect_one()) {
 #pragma unroll 1
@@ -557,6 +545,18 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         __syncwarp();
         if (!OUT) continue;
+        if (!wait(sopready, ph, 15) || !wait(oread, ph ^ 1u, 12)) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          const uint32_t Qc = qtile(c);
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
+                      T::ID_O1, k != 0 ? 1u : 0u);
+          umma_commit(qempty + 8 * (c % T::QBUF));
+          umma_commit(sopread);
+        }
+        __syncwarp();
         // the decayed scores of a half meet v, then the next chunk's scores take their columns (products run in order)
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half) {
