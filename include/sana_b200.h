@@ -258,9 +258,9 @@ int sana_la_rope_take_device_status(int* status_out);
  *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
  *   arguments), 16-byte aligned.
  * State, decays and normalisers are fp32; bf16: both sides of the products are bf16, the state enters the product with q
- * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once.  Bit-reproducible.  A NaN or
- * infinity among the valid tokens reaches every later output of its heads, and may reach outputs up to 15 tokens
- * before it (bf16) in the unnormalised and the normalised form alike.
+ * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once.  Bit-reproducible.  An infinity or
+ * NaN in v gives NaN in its channel from its token on, one in k or q what the sums make of it; no output before the
+ * token is touched.
  *
  * sana_la_decay_step: one token of each of B sequences.  q, k, v, out hold B rows; state [pool, H, D+1, D] is updated in
  * place, row b of the batch using entry slots[b] (slots [B] int32 on the device, or NULL for entry b).  A slot of -1

@@ -43,7 +43,8 @@ struct Lt {
   static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
   static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
   static constexpr int X_BYTES = STACK ? (D + 1) * 32 * (NT == 3 ? 10 : 8) : 0;  // sums of the terms, [D+1][32]; the third in bf16
-  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 4) + (OUT ? 4 * 2 * LT_C : 0) + 8 * 32;
+  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 4) + (OUT ? 4 * 2 * LT_C : 0) + 8 * 32 +
+                                 4 * (4 + 2 * D);
   static constexpr int ONE_EACH = WTILE + VTILE + KTILE + (OUT ? KTILE : 0) + SCRATCH;
   static constexpr int LIMIT = OUT && D <= 32 ? 113 * 1024 : 232448;  // two CTAs per SM, or one
   // a second v tile hides the latency of its load behind the products that still need the first; then one for q
@@ -58,7 +59,10 @@ struct Lt {
   static constexpr int OFF_POW = OFF_X + X_BYTES;        // powers behind 32 zeros
   static constexpr int OFF_RS = OFF_POW + 4 * (32 + LT_C + 4);  // row sums of the scores, [2][128]
   static constexpr int OFF_BAR = OFF_RS + (OUT ? 4 * 2 * LT_C : 0);
-  static constexpr int BYTES = OFF_BAR + 8 * 32;
+  // Tokens whose v is not finite, by channel, for the last chunks: a flag each, then the first such token (128: none).
+  static constexpr int BADS = VBUF == 2 ? 4 : 2;  // a chunk's entries are cleared before the one BADS later can be filled
+  static constexpr int OFF_BAD = OFF_BAR + 8 * 32;
+  static constexpr int BYTES = OFF_BAD + 4 * (4 + BADS * D);
   // Scores in two halves of 64 keys.  O2 has columns of its own, except for 128 channels, where it starts inside the
   // second half and the next chunk's scores wait until it has been read.
   static constexpr bool ALIAS = 128 + 2 * NV + D > 512;
@@ -168,6 +172,9 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  int* bad_flag = reinterpret_cast<int*>(smem + T::OFF_BAD);
+  int* bad_from = bad_flag + 4;
+  for (int i = tid; i < 4 + T::BADS * D; i += T::THREADS) bad_flag[i] = i < 4 ? 0 : C;
   for (int i = tid - 32; i <= C; i += T::THREADS) pow_s[i] = i < 0 ? 0.f : ld_power(gl, i);
   // the ones column of v1 and its padding, once: token t, channels D .. D + 15 = two 16-byte pieces
   for (int i = tid; i < 2 * C * T::VBUF; i += T::THREADS) {
@@ -294,6 +301,20 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         S[NS - 1] = fmaf(whole, S[NS - 1], __uint_as_float(z));
       }
+      volatile int* bad = bad_flag + c % T::BADS;
+      const int* from = bad_from + c % T::BADS * D;
+      const bool poisoned = *bad != 0;  // the same for the four warps: cleared behind their common barrier
+      if (poisoned) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (held(i) && row_of(i) < D && from[row_of(i)] < C) S[i] = __uint_as_float(0x7fffffffu);
+        if (!OUT) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");
+          for (int i = tid; i < D; i += 128) bad_from[c % T::BADS * D + i] = C;
+          if (tid == 0) *bad = 0;
+          __threadfence_block();
+        }
+      }
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dsread);
@@ -328,6 +349,14 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O1 + 16 * (g + 1)), x);
             tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O2 + 16 * (g + 1)), y);
           }
+          if (poisoned) {
+            for (int e = 0; e < 16; ++e)
+              if (t >= from[16 * g + e]) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (k == e >> 1) w[k] |= (e & 1) ? 0x7fff0000u : 0x00007fffu;
+              }
+          }
           if (t < nv) {
             if (a.wide_rows) {  // 32-byte aligned rows: whole sectors
               asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * g), "r"(w[0]), "r"(w[1]),
@@ -338,6 +367,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
           }
           tmem_ld_wait();
+        }
+        if (poisoned) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");
+          for (int i = tid; i < D; i += 128) bad_from[c % T::BADS * D + i] = C;
+          if (tid == 0) *bad = 0;
+          __threadfence_block();
         }
         tcgen05_fence_before();
         __syncwarp();
@@ -491,6 +526,26 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (!live) {  // rows behind the sequence meet zero weights: they must be finite
 #pragma unroll 1
         for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4*>(vt + piece(i * PARTS + part)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      // An infinity or NaN in v would meet the zero scores of the tokens before it: it is taken out here, and the state and
+      // output warps put NaN where it belongs, from its token on.
+#pragma unroll 1
+      for (int i = 0; i < PIECES && live; ++i) {
+        const int ch = i * PARTS + part;
+        const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(ch));
+        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        if (max(m & 0xffffu, m >> 16) >= 0x7f80u) {
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t half = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+            if ((half & 0x7fffu) >= 0x7f80u) {
+              atomicMin(bad_from + c % T::BADS * D + 8 * ch + e, row);
+              w[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+            }
+          }
+          *reinterpret_cast<uint4*>(vt + piece(ch)) = make_uint4(w[0], w[1], w[2], w[3]);
+          bad_flag[c % T::BADS] = 1;
+        }
       }
       if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vt + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
       publish(vfull);
