@@ -529,23 +529,23 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       }
       // An infinity or NaN in v would meet the zero scores of the tokens before it: it is taken out here, and the state and
       // output warps put NaN where it belongs, from its token on.
+      uint32_t big = 0u;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(i * PARTS + part));
+        big = __vmaxu2(big, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+      }
+      if (live && max(big & 0xffffu, big >> 16) >= 0x7f80u) {
 #pragma unroll 1
-      for (int i = 0; i < PIECES && live; ++i) {
-        const int ch = i * PARTS + part;
-        const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(ch));
-        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-        if (max(m & 0xffffu, m >> 16) >= 0x7f80u) {
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t half = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-            if ((half & 0x7fffu) >= 0x7f80u) {
-              atomicMin(bad_from + c % T::BADS * D + 8 * ch + e, row);
-              w[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-            }
+        for (int k = 0; k < 8 * PIECES; ++k) {
+          const int ch = (k >> 3) * PARTS + part;
+          unsigned short* p = reinterpret_cast<unsigned short*>(vt + piece(ch)) + (k & 7);
+          if ((*p & 0x7fffu) >= 0x7f80u) {
+            atomicMin(bad_from + c % T::BADS * D + 8 * ch + (k & 7), row);
+            *p = 0;
           }
-          *reinterpret_cast<uint4*>(vt + piece(ch)) = make_uint4(w[0], w[1], w[2], w[3]);
-          bad_flag[c % T::BADS] = 1;
         }
+        bad_flag[c % T::BADS] = 1;
       }
       if (D % 64 != 0 && part == 0) *reinterpret_cast<uint32_t*>(vt + piece(D / 8)) = 0x3f80u;  // the copy put zeros there
       publish(vfull);
