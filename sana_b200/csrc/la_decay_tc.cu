@@ -634,9 +634,10 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         if (T::ALIAS && ok && c + 1 < chunks) ok = wait(oread, ph, 12) && scores(c + 1, 0) && scores(c + 1, 1);
       }
-    } else if (warp == 9 + LW && lane == 0) {  // copies
+    } else if (warp == 9 + LW) {  // copies; the warp stays together (a lane that waits alone holds up the others' poll for long)
       const int hk = h / a.group;
       auto copy = [&](uint32_t dst, const CUtensorMap* tm, uint32_t full, int head, int n0) {
+        if (!elect_one()) return;
         mbar_expect_tx(full, (uint32_t)T::KTILE);
 #pragma unroll
         for (int i = 0; i < T::KB; ++i)
@@ -647,6 +648,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       };
       // a tile is free only shortly before it is needed again: what it will take is brought into L2 two chunks ahead
       auto prefetch = [&](const CUtensorMap* tm, int head, int n0) {
+        if (!elect_one()) return;
 #pragma unroll
         for (int i = 0; i < T::KB; ++i)
           asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(tm), "r"(64 * i), "r"(head), "r"(n0), "r"(b)
@@ -661,16 +663,19 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (OUT) prefetch(&tmQ, h, n0 + ahead * C);
             prefetch(&tmV, hk, n0 + ahead * C);
           }
-        if (!lt_wait(kempty, ph ^ 1u, abort_flag, 17)) break;
+        if (!__all_sync(0xffffffffu, lt_wait(kempty, ph ^ 1u, abort_flag, 17))) break;
         copy(sm + T::OFF_K, &tmK, kraw, hk, n0);
+        __syncwarp();
         if (OUT) {
           const int qb = c % T::QBUF;
-          if (!lt_wait(qempty + 8 * qb, ((uint32_t)(c / T::QBUF) & 1u) ^ 1u, abort_flag, 18)) break;
+          if (!__all_sync(0xffffffffu, lt_wait(qempty + 8 * qb, ((uint32_t)(c / T::QBUF) & 1u) ^ 1u, abort_flag, 18))) break;
           copy(sm + T::OFF_Q + (uint32_t)(qb * T::KTILE), &tmQ, qraw + 8 * qb, h, n0);
+        __syncwarp();
         }
         const int vb = c % T::VBUF;
-        if (!lt_wait(vempty + 8 * vb, ((uint32_t)(c / T::VBUF) & 1u) ^ 1u, abort_flag, 19)) break;
+        if (!__all_sync(0xffffffffu, lt_wait(vempty + 8 * vb, ((uint32_t)(c / T::VBUF) & 1u) ^ 1u, abort_flag, 19))) break;
         copy(sm + T::OFF_V + (uint32_t)(vb * T::VTILE), &tmV, vraw + 8 * vb, hk, n0);
+        __syncwarp();
       }
     }
   }
