@@ -110,17 +110,18 @@ __device__ __forceinline__ uint32_t lt_ld1(uint32_t taddr) {
 // Bounded wait like mbar_wait, by all lanes of a warp and with the plain poll: the suspend hint of mbar_wait puts the warp
 // to sleep in steps, up to a microsecond past the arrival, and a chunk passes through eight waits in a row.
 __device__ __forceinline__ bool lt_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-  if (mbar_try_wait_poll(bar, parity)) return true;
+  if (__all_sync(0xffffffffu, mbar_try_wait_poll(bar, parity))) return true;
   const long long t0 = clock64();
   uint32_t spins = 0;
-  while (!mbar_try_wait_poll(bar, parity)) {
+  while (!__all_sync(0xffffffffu, mbar_try_wait_poll(bar, parity))) {
     if ((++spins & 255u) == 0) {
-      if (*abort_flag) return false;
-      if (clock64() - t0 > TC_WAIT_LIMIT_CYCLES) {
+      bool stop = *abort_flag != 0;
+      if (!stop && clock64() - t0 > TC_WAIT_LIMIT_CYCLES) {
         *abort_flag = code;
         atomicExch(&g_ld_status, code);
-        return false;
+        stop = true;
       }
+      if (__any_sync(0xffffffffu, stop)) return false;
     }
   }
   return true;
@@ -557,7 +558,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const uint32_t Wu = sm + T::OFF_W, Vu = sm + T::OFF_V, Ku = sm + T::OFF_K, Qu = sm + T::OFF_Q, Su = sm + T::OFF_S;
       const uint64_t sdesc = lt_desc_mn(Su, T::STATE_BLK);
       auto wait = [&](uint32_t bb, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, lt_wait(bb, parity, abort_flag, code));
+        return lt_wait(bb, parity, abort_flag, code);
       };
       auto qtile = [&](int c) -> uint32_t { return Qu + (uint32_t)(c % T::QBUF * T::KTILE); };
       auto scores = [&](int c, int half) -> bool {  // keys 64 half .. + 63 of chunk c
@@ -663,17 +664,17 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (OUT) prefetch(&tmQ, h, n0 + ahead * C);
             prefetch(&tmV, hk, n0 + ahead * C);
           }
-        if (!__all_sync(0xffffffffu, lt_wait(kempty, ph ^ 1u, abort_flag, 17))) break;
+        if (!lt_wait(kempty, ph ^ 1u, abort_flag, 17)) break;
         copy(sm + T::OFF_K, &tmK, kraw, hk, n0);
         __syncwarp();
         if (OUT) {
           const int qb = c % T::QBUF;
-          if (!__all_sync(0xffffffffu, lt_wait(qempty + 8 * qb, ((uint32_t)(c / T::QBUF) & 1u) ^ 1u, abort_flag, 18))) break;
+          if (!lt_wait(qempty + 8 * qb, ((uint32_t)(c / T::QBUF) & 1u) ^ 1u, abort_flag, 18)) break;
           copy(sm + T::OFF_Q + (uint32_t)(qb * T::KTILE), &tmQ, qraw + 8 * qb, h, n0);
         __syncwarp();
         }
         const int vb = c % T::VBUF;
-        if (!__all_sync(0xffffffffu, lt_wait(vempty + 8 * vb, ((uint32_t)(c / T::VBUF) & 1u) ^ 1u, abort_flag, 19))) break;
+        if (!lt_wait(vempty + 8 * vb, ((uint32_t)(c / T::VBUF) & 1u) ^ 1u, abort_flag, 19)) break;
         copy(sm + T::OFF_V + (uint32_t)(vb * T::VTILE), &tmV, vraw + 8 * vb, hk, n0);
         __syncwarp();
       }
