@@ -43,8 +43,8 @@ struct Lt {
   static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
   static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
   static constexpr int X_BYTES = STACK ? (D + 1) * 32 * (NT == 3 ? 10 : 8) : 0;  // sums of the terms, [D+1][32]; the third in bf16
-  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 4) + (OUT ? 4 * 2 * LT_C : 0) + 8 * 32 +
-                                 4 * (4 + 2 * D);
+  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 2 + 32) + (OUT ? 4 * 2 * LT_C : 0) + 240 +
+                                 4 * (4 + 4 * D);
   static constexpr int ONE_EACH = WTILE + VTILE + KTILE + (OUT ? KTILE : 0) + SCRATCH;
   static constexpr int LIMIT = OUT && D <= 32 ? 113 * 1024 : 232448;  // two CTAs per SM, or one
   // a second v tile hides the latency of its load behind the products that still need the first; then one for q
@@ -57,12 +57,12 @@ struct Lt {
   static constexpr int OFF_S = OFF_Q + (OUT ? QBUF * KTILE : 0);
   static constexpr int OFF_X = OFF_S + (OUT ? VB * STATE_BLK : 0);
   static constexpr int OFF_POW = OFF_X + X_BYTES;        // powers behind 32 zeros
-  static constexpr int OFF_RS = OFF_POW + 4 * (32 + LT_C + 4);  // row sums of the scores, [2][128]
+  static constexpr int OFF_RS = OFF_POW + 4 * (32 + LT_C + 2 + 32);  // row sums of the scores, [2][128]
   static constexpr int OFF_BAR = OFF_RS + (OUT ? 4 * 2 * LT_C : 0);
   // Tokens whose v is not finite, by channel, for the last chunks: a flag each, then the first such token (128: none).
   static constexpr int BADS = VBUF == 2 ? 4 : 2;  // a chunk's entries are cleared before the one BADS later can be filled
-  static constexpr int OFF_BAD = OFF_BAR + 8 * 32;
-  static constexpr int BYTES = OFF_BAD + 4 * (4 + BADS * D);
+  static constexpr int OFF_BAD = OFF_BAR + 240;
+  static constexpr int BYTES = OFF_BAD + 4 * (BADS + BADS * D);
   // Scores in two halves of 64 keys.  O2 has columns of its own, except for 128 channels, where it starts inside the
   // second half and the next chunk's scores wait until it has been read.
   static constexpr bool ALIAS = 128 + 2 * NV + D > 512;
@@ -109,6 +109,13 @@ __device__ __forceinline__ uint32_t lt_ld1(uint32_t taddr) {
 
 // Bounded wait like mbar_wait, by all lanes of a warp and with the plain poll: the suspend hint of mbar_wait puts the warp
 // to sleep in steps, up to a microsecond past the arrival, and a chunk passes through eight waits in a row.
+// whether a phase is complete, without waiting
+__device__ __forceinline__ bool lt_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool lt_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait_poll(bar, parity))) return true;
   const long long t0 = clock64();
@@ -150,8 +157,8 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const uint32_t sopread = bar + 120, oready = bar + 128;                                        // 17 of one arrival
   const uint32_t wfull = bar + 136 /* 2 */, vfull = bar + 152, qfull = bar + 160, kfull = bar + 168;
   const uint32_t pready = bar + 176 /* 2 */, rsready = bar + 192 /* 2 */, dsread = bar + 208, sopready = bar + 216, oread = bar + 224;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 240);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 244);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 232);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 236);
 
   const int h = blockIdx.x, seg = blockIdx.y, b = blockIdx.z;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
@@ -169,14 +176,16 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 240), "r"((uint32_t)T::TMEM_COLS)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 232), "r"((uint32_t)T::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   int* bad_flag = reinterpret_cast<int*>(smem + T::OFF_BAD);
-  int* bad_from = bad_flag + 4;
-  for (int i = tid; i < 4 + T::BADS * D; i += T::THREADS) bad_flag[i] = i < 4 ? 0 : C;
+  int* bad_from = bad_flag + T::BADS;
+  for (int i = tid; i < T::BADS + T::BADS * D; i += T::THREADS) bad_flag[i] = i < T::BADS ? 0 : C;
   for (int i = tid - 32; i <= C; i += T::THREADS) pow_s[i] = i < 0 ? 0.f : ld_power(gl, i);
+  float* rev_s = pow_s + C + 2;  // lambda^(31 - k)
+  if (tid < 32) rev_s[tid] = ld_power(gl, 31 - tid);
   // the ones column of v1 and its padding, once: token t, channels D .. D + 15 = two 16-byte pieces
   for (int i = tid; i < 2 * C * T::VBUF; i += T::THREADS) {
     const int t = (i >> 1) % C, ch = D / 8 + (i & 1);
@@ -343,9 +352,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int g = 0; g < D / 16; ++g) {
           uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            w[e] = pack_bf16(fmaf(f, __uint_as_float(x[2 * e]), __uint_as_float(y[2 * e])) * m,
-                             fmaf(f, __uint_as_float(x[2 * e + 1]), __uint_as_float(y[2 * e + 1])) * m);
+          for (int e = 0; e < 8; ++e) {
+            const float2 o = __fmul2_rn(ffma2(make_float2(f, f), make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])),
+                                              make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]))),
+                                        make_float2(m, m));
+            w[e] = pack_bf16(o.x, o.y);
+          }
           if (g + 1 < D / 16) {  // the next columns are under way while these are stored
             tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O1 + 16 * (g + 1)), x);
             tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_O2 + 16 * (g + 1)), y);
@@ -395,7 +407,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       float* rs = reinterpret_cast<float*>(smem + T::OFF_RS) + 32 * w + lane;
       const float* mine = pow_s + lane;
       for (int c = 0; c < chunks; ++c) {
-        float sum = 0.f;
+        float2 sum = make_float2(0.f, 0.f);
         bool ok = true;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {  // rolled: four roles share the instruction cache
@@ -416,25 +428,26 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 const float f = mine[32 * (w - blk) - 31];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                  const float p0 = __uint_as_float(x[2 * e]) * (f * pow_s[31 - 2 * e]);
-                  const float p1 = __uint_as_float(x[2 * e + 1]) * (f * pow_s[30 - 2 * e]);
-                  sum += p0 + p1;
-                  p[e] = pack_bf16(p0, p1);
+                  const float2 d = __fmul2_rn(make_float2(f, f), *reinterpret_cast<const float2*>(rev_s + 2 * e));
+                  const float2 v = __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), d);
+                  sum = __fadd2_rn(sum, v);
+                  p[e] = pack_bf16(v.x, v.y);
                 }
               } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {  // selected, not multiplied by the table's zero: a later token may be NaN
-                  const float p0 = lane >= 2 * e ? __uint_as_float(x[2 * e]) * mine[-2 * e] : 0.f;
-                  const float p1 = lane >= 2 * e + 1 ? __uint_as_float(x[2 * e + 1]) * mine[-2 * e - 1] : 0.f;
-                  sum += p0 + p1;
-                  p[e] = pack_bf16(p0, p1);
+                  const float2 v = __fmul2_rn(make_float2(lane >= 2 * e ? __uint_as_float(x[2 * e]) : 0.f,
+                                                          lane >= 2 * e + 1 ? __uint_as_float(x[2 * e + 1]) : 0.f),
+                                              make_float2(mine[-2 * e], mine[-2 * e - 1]));
+                  sum = __fadd2_rn(sum, v);
+                  p[e] = pack_bf16(v.x, v.y);
                 }
               }
             }
             lt_st16(sc + (uint32_t)(64 * half + 16 * q), p);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          if (half == 1 && a.normalise) rs[(c & 1) * C] = sum;
+          if (half == 1 && a.normalise) rs[(c & 1) * C] = sum.x + sum.y;
           tcgen05_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -613,7 +626,9 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           umma_commit(sopread);
         }
         __syncwarp();
-        // the decayed scores of a half meet v, then the next chunk's scores take their columns (products run in order)
+        // The decayed scores of a half meet v, then the next chunk's scores take their columns (products run in order) - at
+        // once where k and q are there already, else after the other half.
+        bool early = false;
 #pragma unroll 1
         for (int half = 0; half < 2 && ok; ++half) {
           if (!wait(pready + 8 * half, ph, 16)) { ok = false; break; }
@@ -631,8 +646,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
             __syncwarp();
           }
-          if (!T::ALIAS && c + 1 < chunks) ok = scores(c + 1, half);
+          if (!T::ALIAS && half == 0 && c + 1 < chunks) {
+            early = __all_sync(0xffffffffu, lt_test(kfull, ph ^ 1u) && lt_test(qfull, ph ^ 1u));
+            if (early) ok = scores(c + 1, 0);
+          }
         }
+        if (!T::ALIAS && ok && c + 1 < chunks) ok = (early || scores(c + 1, 0)) && scores(c + 1, 1);
         if (T::ALIAS && ok && c + 1 < chunks) ok = wait(oread, ph, 12) && scores(c + 1, 0) && scores(c + 1, 1);
       }
     } else if (warp == 9 + LW) {  // copies; the warp stays together (a lane that waits alone holds up the others' poll for long)
