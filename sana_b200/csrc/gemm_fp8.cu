@@ -69,6 +69,25 @@ __device__ __forceinline__ uint4 f8_scale_words(const F8Scales& s, int r0, int g
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Bounded wait like mbar_wait, with the plain poll: the suspend hint may keep a warp asleep for up to a microsecond past the
+// arrival, and the one accumulator passes from the products to the epilogue and back once a tile.
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (mbar_try_wait_poll(bar, parity)) return true;
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (!mbar_try_wait_poll(bar, parity)) {
+    if ((++spins & 255u) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > TC_WAIT_LIMIT_CYCLES) {
+        *abort_flag = code;
+        atomicExch(&g_fp8_status, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 struct F8Args {
   F8Scales sa, sw;
   int M, N, K;
@@ -109,7 +128,7 @@ __device__ __forceinline__ bool f8_drain(EpiBox& eb, const F8Cols& cols, const E
                                          volatile int* abort_flag) {
   if (nbase >= N) return true;  // uniform
   if (use_res) {
-    if (!mbar_wait(eb.res_bar, eb.res_phase, abort_flag, 5, &g_fp8_status)) return false;
+    if (!f8_wait(eb.res_bar, eb.res_phase, abort_flag, 5)) return false;
     eb.res_phase ^= 1u;
   }
   const bool has_bias = ep.bias != nullptr, has_gate = ep.gate_table != nullptr;
@@ -258,7 +277,7 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
         const int mt = tile / args.tiles_n, nt = tile % args.tiles_n;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1, &g_fp8_status)) { ok = false; break; }
+          if (!f8_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1)) { ok = false; break; }
           const uint32_t sa = tiles_base + stage * S8_STAGE_BYTES;
           const uint32_t fb = bar_full + 8 * stage;
           mbar_expect_tx(fb, S8_STAGE_BYTES);
@@ -274,22 +293,23 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer ---------------------------------------
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, acc_phase = 0u, grp = 0;
-      bool ok = true;
-      int it = 0;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
-        const int a = it & 1;
-        if (!mbar_wait(bar_tempty + 8 * a, ((acc_phase >> a) & 1u) ^ 1u, abort_flag, 2, &g_fp8_status)) { ok = false; break; }
-        acc_phase ^= 1u << a;
+    // the warp waits together and one elected lane issues (see elect_one)
+    uint32_t stage = 0, phase = 0, acc_phase = 0u, grp = 0;
+    bool ok = true;
+    int it = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, f8_wait(bar, parity, abort_flag, code)); };
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+      const int a = it & 1;
+      if (!wait(bar_tempty + 8 * a, ((acc_phase >> a) & 1u) ^ 1u, 2)) break;
+      acc_phase ^= 1u << a;
+      const uint32_t d_tmem = tmem_base + (uint32_t)(a * S8_BN);
+      for (int kb = 0; kb < kblocks; ++kb) {
+        const uint32_t buf = grp & 1u;
+        if ((kb & (F8_GROUP - 1)) == 0 && !wait(bar_sf + 8 * buf, (grp >> 1) & 1u, 6)) { ok = false; break; }
+        if (!wait(bar_full + 8 * stage, phase, 3)) { ok = false; break; }
         tcgen05_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(a * S8_BN);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          const uint32_t buf = grp & 1u;
-          if ((kb & (F8_GROUP - 1)) == 0 &&
-              !mbar_wait(bar_sf + 8 * buf, (grp >> 1) & 1u, abort_flag, 6, &g_fp8_status)) { ok = false; break; }
-          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, 3, &g_fp8_status)) { ok = false; break; }
-          tcgen05_fence_after();
+        const bool last = (kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks;
+        if (elect_one()) {
           const uint32_t sa = tiles_base + stage * S8_STAGE_BYTES;
           const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + S8_A_BYTES);
           const uint32_t sfa_t = tmem_base + (uint32_t)S8_SF_COL0 + 8 * buf, sfb_t = sfa_t + 4;
@@ -298,13 +318,12 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           for (int k = 0; k < 4; ++k)  // 32 elements = 32 bytes inside the 128-byte swizzle row
             umma_fp8(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, sfa_t, sfb_t, (kb | k) != 0 ? 1u : 0u);
           umma_commit(bar_empty + 8 * stage);
-          if ((kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks) {
-            umma_commit(bar_sfempty + 8 * buf);
-            ++grp;
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (last) umma_commit(bar_sfempty + 8 * buf);
+          if (kb + 1 == kblocks) umma_commit(bar_tfull + 8 * a);
         }
-        if (ok) umma_commit(bar_tfull + 8 * a);
+        __syncwarp();
+        if (last) ++grp;
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
     }
   } else if (warp == 2) {
@@ -322,7 +341,7 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           wb = f8_scale_words(args.sw, n0, g + 1, lane);
         }
         // the MMAs that used this buffer are done, and so is the copy that read the shared tile
-        if (!mbar_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7, &g_fp8_status)) ok = false;
+        if (!f8_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         unsigned char* t = sf_gen + buf * 1024 + lane * 16;
         *reinterpret_cast<uint4*>(t) = ca;
@@ -364,7 +383,7 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const bool rows_in = m_box < args.M, use_res = has_res && rows_in;
       f8_box_begin(eb, use_res, lane, m_box, nbase, N, &tmRes);
       const F8Cols cols = f8_cols(ep, m_box, args.M, nbase, N, lane);
-      if (!mbar_wait(bar_tfull + 8 * a, (full_phase >> a) & 1u, abort_flag, 4, &g_fp8_status)) break;
+      if (!f8_wait(bar_tfull + 8 * a, (full_phase >> a) & 1u, abort_flag, 4)) break;
       full_phase ^= 1u << a;
       tcgen05_fence_after();
       uint32_t acc[4][16];
@@ -484,7 +503,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int m0 = mt * 256 + (int)rank * P8_BM;
         const int n0 = nt * P8_BN + (int)rank * (P8_BN / 2);
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1, &g_fp8_status)) { ok = false; break; }
+          if (!f8_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1)) { ok = false; break; }
           const uint32_t sa = tiles_base + stage * P8_STAGE_BYTES;
           if (leader) mbar_expect_tx(bar_full + 8 * stage, 2 * P8_STAGE_BYTES);
           const uint32_t fb = full0 + 8 * stage;
@@ -500,35 +519,36 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer (leader CTA only) -----------------------
-    if (leader && lane == 0) {
+    if (leader) {
       uint32_t stage = 0, phase = 0, acc_phase = 0, grp = 0;
       bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, f8_wait(bar, parity, abort_flag, code)); };
       for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
-        if (!mbar_wait(bar_tempty, acc_phase ^ 1u, abort_flag, 2, &g_fp8_status)) { ok = false; break; }
+        if (!wait(bar_tempty, acc_phase ^ 1u, 2)) break;
         acc_phase ^= 1u;
-        tcgen05_fence_after();
         for (int kb = 0; kb < kblocks; ++kb) {
           const uint32_t buf = grp & 1u;
-          if ((kb & (F8_GROUP - 1)) == 0 &&
-              !mbar_wait(bar_sf + 8 * buf, (grp >> 1) & 1u, abort_flag, 6, &g_fp8_status)) { ok = false; break; }
-          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, 3, &g_fp8_status)) { ok = false; break; }
+          if ((kb & (F8_GROUP - 1)) == 0 && !wait(bar_sf + 8 * buf, (grp >> 1) & 1u, 6)) { ok = false; break; }
+          if (!wait(bar_full + 8 * stage, phase, 3)) { ok = false; break; }
           tcgen05_fence_after();
-          const uint32_t sa = tiles_base + stage * P8_STAGE_BYTES;
-          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + P8_A_BYTES);
-          const uint32_t sfa_t = tmem_base + (uint32_t)P8_SF_COL0 + P8_SF_COLS * buf, sfb_t = sfa_t + 4;
-          const uint32_t idesc = IDESC | f8_scale_byte((uint32_t)(kb & (F8_GROUP - 1)));
+          const bool last = (kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks;
+          if (elect_one()) {
+            const uint32_t sa = tiles_base + stage * P8_STAGE_BYTES;
+            const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + P8_A_BYTES);
+            const uint32_t sfa_t = tmem_base + (uint32_t)P8_SF_COL0 + P8_SF_COLS * buf, sfb_t = sfa_t + 4;
+            const uint32_t idesc = IDESC | f8_scale_byte((uint32_t)(kb & (F8_GROUP - 1)));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_fp8_pair(tmem_base, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, sfa_t, sfb_t,
-                          (kb | k) != 0 ? 1u : 0u);
-          umma_commit_pair(bar_empty + 8 * stage);  // frees this stage in both CTAs
-          if ((kb & (F8_GROUP - 1)) == F8_GROUP - 1 || kb + 1 == kblocks) {
-            tc_commit_pair_local(bar_sfempty + 8 * buf);
-            ++grp;
+            for (int k = 0; k < 4; ++k)
+              umma_fp8_pair(tmem_base, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, sfa_t, sfb_t,
+                            (kb | k) != 0 ? 1u : 0u);
+            umma_commit_pair(bar_empty + 8 * stage);  // frees this stage in both CTAs
+            if (last) tc_commit_pair_local(bar_sfempty + 8 * buf);
+            if (kb + 1 == kblocks) umma_commit_pair(bar_tfull);  // accumulator complete, both CTAs
           }
+          __syncwarp();
+          if (last) ++grp;
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
-        if (ok) umma_commit_pair(bar_tfull);  // accumulator complete, both CTAs
       }
     }
   } else if (warp == 2) {
@@ -545,7 +565,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       for (int g = 0; g < kgroups; ++g, ++grp) {
         const uint32_t buf = grp & 1u, ph = (grp >> 1) & 1u;
         // the copies that read the shared tiles of the group before are done (one commit tells both CTAs)
-        if (grp > 0 && !mbar_wait(bar_sf + 8 * (buf ^ 1u), ((grp - 1) >> 1) & 1u, abort_flag, 8, &g_fp8_status)) ok = false;
+        if (grp > 0 && !f8_wait(bar_sf + 8 * (buf ^ 1u), ((grp - 1) >> 1) & 1u, abort_flag, 8)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         unsigned char* t = sf_gen + lane * 16;
         *reinterpret_cast<uint4*>(t) = wa;
@@ -561,9 +581,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (lane == 0) {
           mbar_arrive_cluster(ready0 + 8 * buf);
           if (leader) {
-            if (!mbar_wait(bar_sfready + 8 * buf, ph, abort_flag, 9, &g_fp8_status)) ok = false;
+            if (!f8_wait(bar_sfready + 8 * buf, ph, abort_flag, 9)) ok = false;
             // the MMAs that used this buffer's columns are done
-            if (ok && !mbar_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7, &g_fp8_status)) ok = false;
+            if (ok && !f8_wait(bar_sfempty + 8 * buf, ph ^ 1u, abort_flag, 7)) ok = false;
             if (ok) {
               tcgen05_fence_after();
               const uint32_t sfa_t = tmem_base + (uint32_t)P8_SF_COL0 + P8_SF_COLS * buf;
@@ -603,7 +623,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const bool rows_in = m_box < args.M, use_res = has_res && rows_in;
       f8_box_begin(eb, use_res, lane, m_box, nbase, N, &tmRes);
       const F8Cols cols = f8_cols(ep, m_box, args.M, nbase, N, lane);
-      if (!mbar_wait(bar_tfull, full_phase, abort_flag, 4, &g_fp8_status)) break;
+      if (!f8_wait(bar_tfull, full_phase, abort_flag, 4)) break;
       full_phase ^= 1u;
       tcgen05_fence_after();
       uint32_t acc[4][16];
