@@ -646,6 +646,76 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   }
 }
 
+// ---- a few rows (single tokens): the weight is streamed once --------------------------------------------------------
+// Bound by the bytes of W: a CTA takes 16 of its rows, its warps split the 128-blocks of K, every load of a warp is
+// 16 bytes and issued before the first is needed.  mma.sync with the W rows as M and the tokens as N (8 a tile): the
+// contraction index may be permuted as long as both operands agree, so a lane's 16 contiguous bytes of a row are the
+// fragments of two instructions.  A block's sum is scaled by 2^(ea + ew) in fp32 and added; the warps' sums meet in
+// shared memory in a fixed order.
+__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d * 2^(s - 254), s the sum of two E8M0 bytes: in two factors, so that neither leaves the range of fp32
+__device__ __forceinline__ float f8_scaled(float d, int s) {
+  const int h = s >> 1;
+  return d * __uint_as_float((uint32_t)h << 23) * __uint_as_float((uint32_t)(s - h) << 23);
+}
+
+template <int NT8, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) gemm_fp8_rows_kernel(const unsigned char* __restrict__ A, const unsigned char* __restrict__ W,
+                                                            __nv_bfloat16* __restrict__ out, int64_t ldo, const F8Args args) {
+  __shared__ float4 red[WARPS][NT8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int n0 = blockIdx.x * 16, K = args.K, kblocks = (K + 127) / 128;
+  const int r0 = n0 + g, r1 = n0 + g + 8;
+  const bool in0 = r0 < args.N, in1 = r1 < args.N;
+  const unsigned char *w0 = W + (int64_t)(in0 ? r0 : 0) * K, *w1 = W + (int64_t)(in1 ? r1 : 0) * K;
+  const unsigned char *s0 = args.sw.p + ((in0 ? r0 : 0) >> args.sw.shift) * args.sw.ld, *s1 = args.sw.p + ((in1 ? r1 : 0) >> args.sw.shift) * args.sw.ld;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  float acc[NT8][4] = {};
+#pragma unroll 2
+  for (int kb = warp; kb < kblocks; kb += WARPS) {
+    const int k = kb * 128 + 16 * c;
+    const bool ka = k < K, kz = k + 64 < K;  // K is a multiple of 16
+    const uint4 wa0 = in0 && ka ? ldg_nc_u4(w0 + k) : zero, wa1 = in1 && ka ? ldg_nc_u4(w1 + k) : zero;
+    const uint4 wz0 = in0 && kz ? ldg_nc_u4(w0 + k + 64) : zero, wz1 = in1 && kz ? ldg_nc_u4(w1 + k + 64) : zero;
+    const int e0 = __ldg(s0 + kb), e1 = __ldg(s1 + kb);
+#pragma unroll
+    for (int t = 0; t < NT8; ++t) {
+      const int m = 8 * t + g;
+      const bool min_ = m < args.M;
+      const unsigned char* x = A + (int64_t)(min_ ? m : 0) * K + k;
+      const uint4 xa = min_ && ka ? __ldg(reinterpret_cast<const uint4*>(x)) : zero;
+      const uint4 xz = min_ && kz ? __ldg(reinterpret_cast<const uint4*>(x + 64)) : zero;
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_e4m3_16832(d, wa0.x, wa1.x, wa0.y, wa1.y, xa.x, xa.y);
+      mma_e4m3_16832(d, wa0.z, wa1.z, wa0.w, wa1.w, xa.z, xa.w);
+      mma_e4m3_16832(d, wz0.x, wz1.x, wz0.y, wz1.y, xz.x, xz.y);
+      mma_e4m3_16832(d, wz0.z, wz1.z, wz0.w, wz1.w, xz.z, xz.w);
+      const int ma = 8 * t + 2 * c, mb = ma + 1;
+      const int f0 = ma < args.M ? __ldg(args.sa.p + (ma >> args.sa.shift) * args.sa.ld + kb) : 127;
+      const int f1 = mb < args.M ? __ldg(args.sa.p + (mb >> args.sa.shift) * args.sa.ld + kb) : 127;
+      acc[t][0] += f8_scaled(d[0], e0 + f0);
+      acc[t][1] += f8_scaled(d[1], e0 + f1);
+      acc[t][2] += f8_scaled(d[2], e1 + f0);
+      acc[t][3] += f8_scaled(d[3], e1 + f1);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT8; ++t) red[warp][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 8 * NT8; i += 32 * WARPS) {
+    const int r = i & 15, m = i >> 4;  // W row of the CTA, token
+    if (m >= args.M || n0 + r >= args.N) continue;
+    const int from = (r & 7) * 4 + ((m & 7) >> 1), word = (r >> 3) * 2 + (m & 1);
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float*>(&red[w][m >> 3][from])[word];
+    out[(int64_t)m * ldo + n0 + r] = from_f32<__nv_bfloat16>(epi_scalar<__nv_bfloat16>(v, m, n0 + r, args.N, args.ep));
+  }
+}
+
 // ---- quantiser --------------------------------------------------------------------------------------------------
 // The least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), from the bits of amax: exponent - 8, one more when the
 // fraction is above 1.75; at least -126 (which a block of zeros takes).  Returns the E8M0 byte e + 127.
@@ -819,6 +889,10 @@ static int launch_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t
   return SANA_OK;
 }
 
+// Most rows the streaming kernel takes: at M = 16 it needs 3.7 - 12.3 us where the tile kernel needs 7.3 - 18 (K x N from
+// 1152 x 1152 to 2240 x 11200); at 24 rows 17 against 10.5 us (2240 x 6720).
+constexpr int64_t F8_ROWS = 16;
+
 template <int ACT>
 static int launch_gemm_fp8(bool pair, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
                            const CUtensorMap& tmRes, F8Args& a, cudaStream_t st) {
@@ -890,6 +964,20 @@ extern "C" int sana_gemm_fp8(const void* Aq, const void* sfa, int64_t ldsfa, int
   a.sw = {static_cast<const unsigned char*>(sfw), ldsfw, N, w_block_rows == 128 ? 7 : 0};
   a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.ep = p;
+  if (M <= F8_ROWS && gemm_variant() == 0) {
+    const unsigned char *ap = static_cast<const unsigned char*>(Aq), *wp = static_cast<const unsigned char*>(Wq);
+    __nv_bfloat16* op = static_cast<__nv_bfloat16*>(out);
+    const unsigned grid = (unsigned)ceil_div(N, 16);
+    // 16 warps a CTA while every CTA has an SM of its own (M = 1: N = 1152 3.2 us against 4.2 with eight, N = 2240, K = 5600
+    // 6.8 against 9.0); eight beyond, where several share one (N = 6720 6.5 against 9.1, N = 11200 9.8 against 12.6)
+    const bool wide = ceil_div(N, 16) <= sm_count();
+    if (M <= 8 && wide) gemm_fp8_rows_kernel<1, 16><<<grid, 512, 0, st>>>(ap, wp, op, ldo, a);
+    else if (M <= 8) gemm_fp8_rows_kernel<1, 8><<<grid, 256, 0, st>>>(ap, wp, op, ldo, a);
+    else if (wide) gemm_fp8_rows_kernel<2, 16><<<grid, 512, 0, st>>>(ap, wp, op, ldo, a);
+    else gemm_fp8_rows_kernel<2, 8><<<grid, 256, 0, st>>>(ap, wp, op, ldo, a);
+    SANA_LAUNCH_CHECK("gemm_fp8_rows kernel");
+    return SANA_OK;
+  }
   CUtensorMap tmA, tmB, tmOut, tmRes;
   rc = make_tmap_2d(&tmOut, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, M, N, ldo * 2, 32, EPI_BOX_COLS);
   if (rc) return rc;

@@ -721,6 +721,14 @@ def take_gemm_nvfp4_device_status() -> int:
 
 FP8_BLOCK = 128  # elements along K that share a scale
 
+# The single-token operators below are bound by the host, and looking up the current stream through its Python object is a
+# tenth of such a call: the raw handle where torch offers it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(device_index: int) -> int:
+    return _raw_stream(device_index) if _raw_stream is not None else _stream()
+
 
 def _device_of(what: str, *ts: Optional[torch.Tensor]) -> int:
     """Index of the one CUDA device that all given tensors live on."""
@@ -728,11 +736,12 @@ def _device_of(what: str, *ts: Optional[torch.Tensor]) -> int:
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise SanaLibraryError("sana_b200 operators run on CUDA tensors only (no CPU path)")
         if index < 0:
-            index = t.device.index
-        elif t.device.index != index:
+            index = i
+        elif i != index:
             raise SanaLibraryError(f"{what}: tensors on different devices")
     return index
 
@@ -765,6 +774,13 @@ class Fp8Tensor:
             scales = padded[:, :kb]
         self.q, self.scales, self.block_rows = q, scales, block_rows
 
+    @classmethod
+    def _of(cls, q: torch.Tensor, scales: torch.Tensor, block_rows: int, rows: int, K: int) -> "Fp8Tensor":
+        """From buffers that are known to be right (the quantiser's own)."""
+        t = cls.__new__(cls)
+        t.q, t.scales, t.block_rows, t.rows, t.K = q, scales, block_rows, rows, K
+        return t
+
     def dequantize(self) -> torch.Tensor:
         """fp32 [rows, K] reconstruction (torch math; for tests and diagnostics only)."""
         e = self.scales.to(torch.int32).repeat_interleave(self.block_rows, 0)[:self.rows]
@@ -789,9 +805,9 @@ def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
     words = (kb + 3) // 4 * 4
     sf = torch.empty((rows + block_rows - 1) // block_rows, words, dtype=torch.uint8, device=x.device)
     _lib.check(_lib.load().sana_fp8_quantize(x.data_ptr(), ld if rows > 1 else max(ld, K), q.data_ptr(), sf.data_ptr(), words,
-                                             rows, K, block_rows, _dtype_code(x.dtype), _stream()), "sana_fp8_quantize")
+                                             rows, K, block_rows, _dtype_code(x.dtype), _stream_of(dev)), "sana_fp8_quantize")
     counters.launches += 1
-    return Fp8Tensor(q, sf[:, :kb], block_rows)
+    return Fp8Tensor._of(q, sf[:, :kb], block_rows, rows, K)
 
 
 def gemm_fp8(a: Fp8Tensor, w: Fp8Tensor, bias=None, act: int = ACT_NONE, relu_cols: int = 0, gate=None,
@@ -810,10 +826,12 @@ def gemm_fp8(a: Fp8Tensor, w: Fp8Tensor, bias=None, act: int = ACT_NONE, relu_co
     Mo, No, ldo = _rows2d(out, "gemm_fp8 out")
     if Mo != M or No != Nn or out.dtype != torch.bfloat16:
         raise SanaLibraryError("gemm_fp8: bad output tensor")
-    ep, keep = _epilogue(M, Nn, torch.bfloat16, bias, act, relu_cols, gate, residual)
+    ep = keep = None
+    if bias is not None or act != ACT_NONE or gate is not None or residual is not None:
+        ep, keep = _epilogue(M, Nn, torch.bfloat16, bias, act, relu_cols, gate, residual)
     _lib.check(_lib.load().sana_gemm_fp8(a.q.data_ptr(), a.scales.data_ptr(), a.scales.stride(0), a.block_rows, w.q.data_ptr(),
                                          w.scales.data_ptr(), w.scales.stride(0), w.block_rows, out.data_ptr(), ldo, M, Nn, K,
-                                         C.byref(ep), _stream()), "sana_gemm_fp8")
+                                         C.byref(ep) if ep is not None else None, _stream_of(dev)), "sana_gemm_fp8")
     counters.launches += 1
     return out
 
@@ -888,7 +906,7 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
     _lib.check(lib.sana_la_decay(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
                                  prior.data_ptr() if prior is not None else None, lens, state.data_ptr(), out.data_ptr(), ldo,
                                  ws.data_ptr() if ws is not None else None, ws_bytes, B, N, H, Hk, D, scale, 1 if relu else 0,
-                                 -1.0 if eps is None else eps, dt, _stream()), "sana_la_decay")
+                                 -1.0 if eps is None else eps, dt, _stream_of(dev)), "sana_la_decay")
     counters.launches += 2 if ws_bytes else 1
     return out, state
 
@@ -921,7 +939,7 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
     _lib.check(_lib.load().sana_la_decay_step(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
                                               state.data_ptr(), state.shape[0], ids, out.data_ptr(), ldo if B > 1 else max(ldo, co),
                                               B, H, Hk, D, scale, 1 if relu else 0, -1.0 if eps is None else eps,
-                                              _dtype_code(q.dtype), _stream()), "sana_la_decay_step")
+                                              _dtype_code(q.dtype), _stream_of(dev)), "sana_la_decay_step")
     counters.launches += 1
     return out
 
