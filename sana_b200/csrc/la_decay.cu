@@ -11,23 +11,25 @@
 // Powers of lambda are always taken at the difference of two positions (never lambda^t * lambda^-s, which overflows for
 // a strong decay).
 //
-// bf16 kernel: a CTA walks the chunks of one token segment of one head (narrow heads: several heads a CTA) with the
-// state in the accumulator registers of its warps: warp w owns value channels 16 w .. 16 w + 15 against all key
-// channels.  The accumulator fragment of S is, register for register, the B operand of S phi(q) (rows of S are the
-// columns of the product), and the transposed fragment of v that multiplies the probabilities is the A operand of the
-// state update, so the state never moves and v is read from shared memory once.
+// bf16, more than 64 tokens: la_decay_tc.cu.  bf16 kernel here: prompts of at most 64 tokens, one chunk, a CTA for one head
+// (narrow heads: several), bound by latency - it starts and ends faster than the tensor-memory kernels' pipeline (64 tokens:
+// 8 x 70 heads of 32 channels 10 us against 16, 8 x 16 heads of 128 14 against 21; 20 heads of 112 12 against 11).  The state lives in the accumulator
+// registers of the warps: warp w owns value channels 16 w .. 16 w + 15 against all key channels.  The accumulator fragment
+// of S is, register for register, the B operand of S phi(q) (rows of S are the columns of the product), and the transposed
+// fragment of v that multiplies the scores is the A operand of the state update, so the state never moves and v is read
+// from shared memory once.
 // The state stays within a few 2^-24 of fp32: the weighted v is split into three bf16 terms (8 bits each) before the
 // tensor core sees it.  In S phi(q) the state enters as two bf16 terms (2^-16); the scores are rounded to bf16 once,
 // like the output.  The normaliser is summed in fp32 from the unrounded scores.
-// A sequence is split over CTAs into segments when there are fewer heads than the GPU has room for: a first launch
-// computes what each segment adds to the state, and each CTA of the second combines those of the segments before its
-// own, in order (nothing depends on the order in which CTAs run).
+// fp32: the chunked form on the CUDA cores.  A sequence is split over CTAs into segments when there are fewer heads than the
+// GPU has room for: a first launch computes what each segment adds to the state, and each CTA of the second combines those
+// of the segments before its own, in order (nothing depends on the order in which CTAs run).
 #include "la_decay.cuh"
 
 namespace sana {
 
-constexpr int LD_C = 64;  // tokens per chunk, bf16
-constexpr int LD_CF = 32;  // fp32
+constexpr int LD_C = 64;   // most tokens of the bf16 kernel
+constexpr int LD_CF = 32;  // tokens per chunk, fp32
 
 __device__ __forceinline__ void ld_cp16(uint32_t dst, const void* src, bool valid) {
   const int sz = valid ? 16 : 0;
@@ -54,18 +56,18 @@ struct Ld {
   static constexpr int ROW = 2 * D + 16;                   // odd number of 16-byte pieces: ldmatrix without conflicts
   static constexpr int TILE = LD_C * ROW;
   static constexpr int PROW = 2 * LD_C + 16;               // scores; the 16 spare bytes hold the four partial row sums
-  static constexpr int OFF_P = 6 * TILE;                   // [2][q, k, v] | scores | powers | key sum | q . key sum
+  static constexpr int OFF_P = 3 * TILE;                   // q, k, v | scores | powers | key sum | q . key sum |
   static constexpr int OFF_POW = OFF_P + LD_C * PROW;
   static constexpr int OFF_Z = OFF_POW + 4 * (LD_C + 4);
   static constexpr int OFF_QZ = OFF_Z + 4 * D;
-  static constexpr int HEAD_BYTES = OFF_QZ + 4 * LD_C;
+  static constexpr int OFF_BAD = OFF_QZ + 4 * LD_C;         // first token whose v is not finite, by channel
+  static constexpr int HEAD_BYTES = OFF_BAD + 4 * D;
   static constexpr int BYTES = HG * HEAD_BYTES;
   static_assert(HEAD_BYTES % 16 == 0, "tiles stay 16-byte aligned");
 };
 
-// OUT: outputs and (last segment) the final state; else: what the segment adds to the state.
-template <int D, bool OUT>
-__global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdArgs a) {
+template <int D>
+__global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_short_kernel(const LdArgs a) {
   using T = Ld<D>;
   constexpr int WH = T::WH, KT = D / 16, C = LD_C;
   extern __shared__ __align__(16) unsigned char smem_all[];
@@ -76,36 +78,31 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
   float* pow_s = reinterpret_cast<float*>(smem + T::OFF_POW);
   float* z_s = reinterpret_cast<float*>(smem + T::OFF_Z);
   float* qz_s = reinterpret_cast<float*>(smem + T::OFF_QZ);
-  const int h = blockIdx.x * T::HG + hg, seg = blockIdx.y, b = blockIdx.z;
+  int* bad_s = reinterpret_cast<int*>(smem + T::OFF_BAD);
+  const int h = blockIdx.x * T::HG + hg, b = blockIdx.z;
   const bool active = h < a.H;  // inactive head groups of the last CTA only keep the barriers
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
-  const int seg_begin = seg * a.seg_len, seg_end = min(a.N, seg_begin + a.seg_len);
-  const int n_begin = min(seg_begin, len), n_end = min(seg_end, len);
+  const int nv = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
   const float gl = active ? a.log_decay[h] : 0.f;
   const int hk = h / a.group;
   const int64_t row0 = (int64_t)b * a.N;
-  const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(a.q) + row0 * a.ldq + (int64_t)h * D;
-  const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.k) + row0 * a.ldk + (int64_t)hk * D;
-  const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.v) + row0 * a.ldv + (int64_t)hk * D;
   const bool relu = a.relu != 0;
-
-  auto load = [&](int n0, int buf) {
-    if (active) {
-      const uint32_t base = sm + buf * 3 * T::TILE;
-      for (int i = tid; i < C * (D / 8); i += 32 * WH) {
-        const int r = i / (D / 8), ch = i % (D / 8), tok = n0 + r;
-        const bool ok = tok < n_end;
-        const int64_t t = ok ? tok : n_begin;  // a valid address; nothing is read from it
-        const uint32_t dst = base + r * T::ROW + ch * 16;
-        if (OUT) ld_cp16(dst, qp + t * a.ldq + 8 * ch, ok);
-        ld_cp16(dst + T::TILE, kp + t * a.ldk + 8 * ch, ok);
-        ld_cp16(dst + 2 * T::TILE, vp + t * a.ldv + 8 * ch, ok);
-      }
+  if (active) {
+    const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(a.q) + row0 * a.ldq + (int64_t)h * D;
+    const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.k) + row0 * a.ldk + (int64_t)hk * D;
+    const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.v) + row0 * a.ldv + (int64_t)hk * D;
+    for (int i = tid; i < C * (D / 8); i += 32 * WH) {
+      const int r = i / (D / 8), ch = i % (D / 8);
+      const bool ok = r < nv;
+      const int64_t t = ok ? r : 0;  // a valid address; nothing is read from it
+      const uint32_t dst = sm + r * T::ROW + ch * 16;
+      ld_cp16(dst, qp + t * a.ldq + 8 * ch, ok);
+      ld_cp16(dst + T::TILE, kp + t * a.ldk + 8 * ch, ok);
+      ld_cp16(dst + 2 * T::TILE, vp + t * a.ldv + 8 * ch, ok);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if (n_begin < n_end) load(n_begin, 0);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
   for (int i = tid; i <= C; i += 32 * WH) pow_s[i] = ld_power(gl, i);
+  for (int i = tid; i < D; i += 32 * WH) bad_s[i] = C;
 
   // state: rows 16 wh + g and + 8 (value channels), columns 8 n + c2, + 1 (key channels); zacc: rows 0..2 hold the three
   // terms of the key sum of columns 16 wh + 8 n + c2, + 1
@@ -119,35 +116,24 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
 #pragma unroll
     for (int e = 0; e < 4; ++e) zacc[n][e] = 0.f;
   const int64_t per = (int64_t)(D + 1) * D;
-  if (OUT && active) {  // the state before this segment
-    auto add = [&](const float* src, float f) {
-      const float* r = src + (int64_t)(16 * wh + g) * D + c2;
+  if (a.prior && active) {
+    const float* src = a.prior + ((int64_t)b * a.H + h) * per;
+    const float* r = src + (int64_t)(16 * wh + g) * D + c2;
 #pragma unroll
-      for (int n = 0; n < 2 * KT; ++n) {
-        const float2 u = __ldg(reinterpret_cast<const float2*>(r + 8 * n));
-        const float2 w = __ldg(reinterpret_cast<const float2*>(r + 8 * D + 8 * n));
-        S[n][0] = fmaf(f, u.x, S[n][0]);
-        S[n][1] = fmaf(f, u.y, S[n][1]);
-        S[n][2] = fmaf(f, w.x, S[n][2]);
-        S[n][3] = fmaf(f, w.y, S[n][3]);
-      }
-      if (g == 0) {
+    for (int n = 0; n < 2 * KT; ++n) {
+      const float2 u = __ldg(reinterpret_cast<const float2*>(r + 8 * n));
+      const float2 w = __ldg(reinterpret_cast<const float2*>(r + 8 * D + 8 * n));
+      S[n][0] = u.x, S[n][1] = u.y, S[n][2] = w.x, S[n][3] = w.y;
+    }
+    if (g == 0) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float2 u = __ldg(reinterpret_cast<const float2*>(src + (int64_t)D * D + 16 * wh + 8 * n + c2));
-          zacc[n][0] = fmaf(f, u.x, zacc[n][0]);
-          zacc[n][1] = fmaf(f, u.y, zacc[n][1]);
-        }
+      for (int n = 0; n < 2; ++n) {
+        const float2 u = __ldg(reinterpret_cast<const float2*>(src + (int64_t)D * D + 16 * wh + 8 * n + c2));
+        zacc[n][0] = u.x, zacc[n][1] = u.y;
       }
-    };
-    if (a.prior) add(a.prior + ((int64_t)b * a.H + h) * per, ld_power(gl, n_begin));
-    for (int r = 0; r < seg; ++r) {
-      const int end = min((r + 1) * a.seg_len, len);
-      if (end == min(r * a.seg_len, len)) break;  // past the sequence: these segments hold nothing
-      add(a.partial + (((int64_t)b * a.npart + r) * a.H + h) * per, ld_power(gl, n_begin - end));
     }
   }
-  auto publish_z = [&]() {  // the key sum into shared memory: the three terms are rows 0, 1, 2 = lanes 4 g
+  {  // the key sum into shared memory: the three terms are rows 0, 1, 2 = lanes 4 g
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -156,20 +142,39 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
         z += __shfl_down_sync(0xffffffffu, zacc[n][e], 4) + __shfl_down_sync(0xffffffffu, zacc[n][e], 8);
         if (g == 0) z_s[16 * wh + 8 * n + c2 + e] = z;
       }
-  };
-  if (OUT) publish_z();
+  }
 
   // ldmatrix addresses inside a tile: 16 rows x 16 columns as four 8 x 8 matrices
   const uint32_t off_rows = (lane & 15) * T::ROW + (lane >> 4) * 16;                       // (rows 0-7, 8-15) x (columns 0-7, 8-15)
   const uint32_t off_cols = ((lane & 7) + (lane >> 4) * 8) * T::ROW + ((lane >> 3) & 1) * 16;  // columns first
-  int buf = 0;
-  for (int n0 = n_begin; n0 < n_end; n0 += C, buf ^= 1) {
-    const int nv = min(C, n_end - n0);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the tiles of this chunk are there, and everybody is done with the chunk before
-    if (n0 + C < n_end) load(n0 + C, buf ^ 1);
-    const uint32_t Qs = sm + buf * 3 * T::TILE, Ks = Qs + T::TILE, Vs = Ks + T::TILE, Ps = sm + T::OFF_P;
-    if (OUT) {
+  const uint32_t Qs = sm, Ks = Qs + T::TILE, Vs = Ks + T::TILE, Ps = sm + T::OFF_P;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  // An infinity or NaN in v would meet the zero scores of the tokens before it: it is taken out, and NaN put where it belongs.
+  bool odd = false;
+  if (active) {
+    for (int i = tid; i < C * (D / 8); i += 32 * WH) {  // the pieces this thread has loaded
+      const int r = i / (D / 8), ch = i % (D / 8);
+      unsigned short* p = reinterpret_cast<unsigned short*>(smem + 2 * T::TILE + r * T::ROW + ch * 16);
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+      odd |= max(m & 0xffffu, m >> 16) >= 0x7f80u;
+    }
+  }
+  odd = __syncthreads_or(odd);  // the tiles are there
+  if (odd) {
+    if (active)
+      for (int i = tid; i < C * D; i += 32 * WH) {
+        const int r = i / D, ch = i % D;
+        unsigned short* p = reinterpret_cast<unsigned short*>(smem + 2 * T::TILE + r * T::ROW) + ch;
+        if ((*p & 0x7fffu) >= 0x7f80u) {
+          atomicMin(bad_s + ch, r);
+          *p = 0;
+        }
+      }
+    __syncthreads();
+  }
+  {
+    {
       if (active) {
         // scores of the 16 x 16 blocks on and below the diagonal, dealt to the warps in turn
         int id = 0;
@@ -237,11 +242,11 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
       }
       __syncthreads();  // scores and normalisers are there
     }
-    if (!active) continue;
+    if (!active) return;
     uint32_t vf[4][4];  // v of the chunk, this warp's 16 channels: [token tile][(s 0-7, ch 0-7), (s 8-15, 0-7), (0-7, 8-15), (8-15, 8-15)]
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) ldsm_x4_t(vf[kt], Vs + kt * 16 * T::ROW + off_rows + wh * 32);
-    if (OUT) {
+    {
       float o[4][2][4] = {};
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {  // S phi(q): key channels 16 kt ..
@@ -291,6 +296,14 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
           m0 = 1.f / (d0 + a.eps);
           m1 = 1.f / (d1 + a.eps);
         }
+        if (odd) {
+          const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * mi + g + 8 * (e >> 1) >= bad_s[16 * wh + 8 * r + c2 + (e & 1)]) o[mi][r][e] = nan;
+        }
         // the four lanes of a row group swap so that each holds 16 bytes of one row: lane 0 / 1 row g, channels 0-7 / 8-15,
         // lane 2 / 3 the same of row g + 8
         uint32_t w[4] = {pack_bf16(o[mi][0][0] * m0, o[mi][0][1] * m0), pack_bf16(o[mi][1][0] * m0, o[mi][1][1] * m0),
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
         }
         const int t = 16 * mi + g + 8 * (c >> 1);
         if (t < nv)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + n0 + t) * a.ldo + (int64_t)h * D + 16 * wh +
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 16 * wh +
                                     8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
@@ -364,34 +377,32 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_bf16_kernel(const LdA
           for (int e = 0; e < 2; ++e) zacc[r][e] = fmaf(whole, zacc[r][e], z[r][e]);
       }
     }
-    if (OUT) publish_z();
   }
-  if (!active) return;
-
-  if (!OUT || seg == a.nseg - 1) {
-    float* dst = OUT ? a.state + ((int64_t)b * a.H + h) * per : a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
-    float* r = dst + (int64_t)(16 * wh + g) * D + c2;
+  if (odd) {
 #pragma unroll
-    for (int n = 0; n < 2 * KT; ++n) {
-      *reinterpret_cast<float2*>(r + 8 * n) = make_float2(S[n][0], S[n][1]);
-      *reinterpret_cast<float2*>(r + 8 * D + 8 * n) = make_float2(S[n][2], S[n][3]);
-    }
+    for (int n = 0; n < 2 * KT; ++n)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float z[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        z[e] = zacc[n][e] + __shfl_down_sync(0xffffffffu, zacc[n][e], 4) + __shfl_down_sync(0xffffffffu, zacc[n][e], 8);
-      if (g == 0) *reinterpret_cast<float2*>(dst + (int64_t)D * D + 16 * wh + 8 * n + c2) = make_float2(z[0], z[1]);
-    }
+      for (int e = 0; e < 4; ++e)
+        if (bad_s[16 * wh + g + 8 * (e >> 1)] < C) S[n][e] = __uint_as_float(0x7fffffffu);
   }
-  if (OUT) {  // rows of the segment past the sequence are zeros
-    const int z0 = max(seg_begin, n_end);
-    for (int64_t i = tid; i < (int64_t)max(0, seg_end - z0) * (D / 8); i += 32 * WH) {
-      const int t = z0 + (int)(i / (D / 8)), ch = (int)(i % (D / 8));
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 8 * ch) =
-          make_uint4(0u, 0u, 0u, 0u);
-    }
+  float* dst = a.state + ((int64_t)b * a.H + h) * per;
+  float* r = dst + (int64_t)(16 * wh + g) * D + c2;
+#pragma unroll
+  for (int n = 0; n < 2 * KT; ++n) {
+    *reinterpret_cast<float2*>(r + 8 * n) = make_float2(S[n][0], S[n][1]);
+    *reinterpret_cast<float2*>(r + 8 * D + 8 * n) = make_float2(S[n][2], S[n][3]);
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    float z[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      z[e] = zacc[n][e] + __shfl_down_sync(0xffffffffu, zacc[n][e], 4) + __shfl_down_sync(0xffffffffu, zacc[n][e], 8);
+    if (g == 0) *reinterpret_cast<float2*>(dst + (int64_t)D * D + 16 * wh + 8 * n + c2) = make_float2(z[0], z[1]);
+  }
+  for (int i = tid; i < (a.N - nv) * (D / 8); i += 32 * WH) {  // rows past the sequence are zeros
+    const int t = nv + i / (D / 8), ch = i % (D / 8);
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 8 * ch) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -611,32 +622,33 @@ __global__ void __launch_bounds__(256) la_decay_step_kernel(const LdStepArgs a) 
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-// CTAs resident at once on the current device; also raises the kernels' shared-memory limits there, once.
+// CTAs of the fp32 kernel resident at once on the current device; also raises its shared-memory limit there, once.
 template <int D>
-static int64_t ld_slots(int dtype) {
-  static int64_t known[64][2] = {};
+static int64_t ld_slots() {
+  static int64_t known[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  int64_t& n = known[dev][dtype == SANA_BF16];
-  if (n > 0) return n;
-  if (dtype == SANA_BF16) {
-    cudaFuncSetAttribute(la_decay_bf16_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ld<D>::BYTES);
-    cudaFuncSetAttribute(la_decay_bf16_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ld<D>::BYTES);
-    return n = resident_ctas(la_decay_bf16_kernel<D, true>, Ld<D>::THREADS, Ld<D>::BYTES);
-  }
+  if (known[dev] > 0) return known[dev];
   cudaFuncSetAttribute(la_decay_f32_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LdF<D>::FLOATS * 4);
   cudaFuncSetAttribute(la_decay_f32_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, LdF<D>::FLOATS * 4);
-  return n = resident_ctas(la_decay_f32_kernel<D, true>, 256, LdF<D>::FLOATS * 4);
+  return known[dev] = resident_ctas(la_decay_f32_kernel<D, true>, 256, LdF<D>::FLOATS * 4);
 }
 
-// Token segments: a sequence is cut only when the heads alone leave the GPU partly empty, since every cut re-reads k and
-// v.  Cost of a choice = waves x (tokens of a segment, plus half as many again for the first launch, plus about two
-// chunks for reading the states before it).
+constexpr int64_t LD_TC_TOKENS = LD_C + 1;  // shortest sequences the tcgen05 kernels take
+
+// Token segments and their number; npart = segments whose sums go through the workspace.  fp32: a sequence is cut only when
+// the heads alone leave the GPU partly empty, since every cut re-reads k and v.  Cost of a choice = waves x (tokens of a
+// segment, plus half as many again for the first launch, plus about two chunks for reading the states before it).
 template <int D>
-static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, int* nseg) {
-  const int C = dtype == SANA_BF16 ? LD_C : LD_CF;
-  const int64_t units = B * (dtype == SANA_BF16 ? ceil_div(H, Ld<D>::HG) : H), slots = ld_slots<D>(dtype);
-  const int64_t chunks = ceil_div(N, C);
+static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, int* nseg, int* npart) {
+  if (dtype == SANA_BF16) {
+    LdPlan p = {LD_C, 1};
+    *npart = 0;
+    if (N >= LD_TC_TOKENS) p = ld_tc_plan(B, N, H, D, npart);
+    *seg_len = p.seg_len, *nseg = p.nseg;
+    return;
+  }
+  const int64_t units = B * H, slots = ld_slots<D>(), chunks = ceil_div(N, LD_CF);
   int64_t best = -1, best_len = chunks;
   for (int64_t n = 1; n <= chunks && n <= 64; ++n) {
     const int64_t len = ceil_div(chunks, n), real = ceil_div(chunks, len);
@@ -644,36 +656,23 @@ static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, in
     if (real > 1) cost += ceil_div(units * (real - 1), slots) * len + 4 + real;
     if (best < 0 || cost < best) best = cost, best_len = len;
   }
-  *seg_len = (int)(best_len * C);
+  *seg_len = (int)(best_len * LD_CF);
   *nseg = (int)ceil_div(N, (int64_t)*seg_len);
-}
-
-constexpr int64_t LD_TC_TOKENS = 65;  // shortest sequences the tcgen05 kernels take
-
-template <int D>
-static void ld_any_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, int* nseg, int* npart) {
-  if (dtype == SANA_BF16 && N >= LD_TC_TOKENS) {
-    const LdPlan p = ld_tc_plan(B, N, H, D, npart);
-    *seg_len = p.seg_len;
-    *nseg = p.nseg;
-  } else {
-    ld_plan<D>(B, N, H, dtype, seg_len, nseg);
-    *npart = *nseg - 1;
-  }
+  *npart = *nseg - 1;
 }
 
 template <int D>
 static int launch_decay(LdArgs& a, int64_t B, int dtype, int64_t workspace_bytes, cudaStream_t st) {
-  ld_any_plan<D>(B, a.N, a.H, dtype, &a.seg_len, &a.nseg, &a.npart);
+  ld_plan<D>(B, a.N, a.H, dtype, &a.seg_len, &a.nseg, &a.npart);
   SANA_REQUIRE(workspace_bytes >= (int64_t)4 * B * a.npart * a.H * (D + 1) * D, "sana_la_decay: workspace too small");
-  if (dtype == SANA_BF16 && a.N >= LD_TC_TOKENS) return launch_decay_tc(a, B, D, st);
   if (dtype == SANA_BF16) {
-    const dim3 grid((unsigned)ceil_div(a.H, Ld<D>::HG), (unsigned)a.nseg, (unsigned)B);
-    if (a.nseg > 1) {
-      la_decay_bf16_kernel<D, false><<<dim3(grid.x, a.nseg - 1, grid.z), Ld<D>::THREADS, Ld<D>::BYTES, st>>>(a);
-      SANA_LAUNCH_CHECK("la_decay segment kernel");
+    if (a.N >= LD_TC_TOKENS) return launch_decay_tc(a, B, D, st);
+    static OncePerDevice once;
+    if (once.first_time()) {
+      cudaError_t e = cudaFuncSetAttribute(la_decay_short_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ld<D>::BYTES);
+      if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(la_decay_short)");
     }
-    la_decay_bf16_kernel<D, true><<<grid, Ld<D>::THREADS, Ld<D>::BYTES, st>>>(a);
+    la_decay_short_kernel<D><<<dim3((unsigned)ceil_div(a.H, Ld<D>::HG), 1, (unsigned)B), Ld<D>::THREADS, Ld<D>::BYTES, st>>>(a);
   } else {
     const dim3 grid((unsigned)a.H, (unsigned)a.nseg, (unsigned)B);
     if (a.nseg > 1) {
@@ -729,7 +728,7 @@ using namespace sana;
 extern "C" int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype) {
   if (B <= 0 || N <= 0 || N >= ((int64_t)1 << 30) || H <= 0 || !ld_head_dim(D) || (dtype != SANA_BF16 && dtype != SANA_F32)) return -1;
   int len = 0, nseg = 1, npart = 0;
-  LD_DISPATCH(D, (ld_any_plan<HD>(B, N, H, dtype, &len, &nseg, &npart)));
+  LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, &len, &nseg, &npart)));
   return (int64_t)4 * B * npart * H * (D + 1) * D;
 }
 

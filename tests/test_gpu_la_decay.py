@@ -176,6 +176,37 @@ def test_non_finite_values_stay_behind_their_token(dtype, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D,N,at", [(16, 40, 20), (32, 64, 37), (48, 200, 131), (64, 300, 257), (96, 129, 128), (112, 2000, 1111), (128, 700, 5)])
+def test_no_output_depends_on_a_later_token(dtype, D, N, at):
+    B, H = 1, 2
+    kw = dict(relu=True, eps=1e-8)
+    q, k, v, ld, _ = make(B, N, H, D, dtype)
+    clean, _ = ops.la_decay(q, k, v, ld, B, N, H, D, **kw)
+    for value in (float("nan"), float("-inf"), 1e4):
+        for t in (k, v):
+            old = t[at:].clone()
+            t[at:] = value
+            out, st = ops.la_decay(q, k, v, ld, B, N, H, D, **kw)
+            assert torch.equal(out[:at], clean[:at])
+            assert math.isfinite(value) or not torch.isfinite(st).all() or t is k
+            t[at:] = old
+        # one channel of one token: its channel from there on, nothing else
+        old = v[at, 3].clone()
+        v[at, 3] = value
+        out, st = ops.la_decay(q, k, v, ld, B, N, H, D, **kw)
+        same = torch.ones_like(clean, dtype=torch.bool)
+        same[at:, 3] = False
+        assert torch.equal(out[same], clean[same])
+        if not math.isfinite(value):
+            live = (q[at:, :D].float().clamp(min=0) * k[at, :D].float().clamp(min=0)).sum(-1) > 0
+            assert not torch.isfinite(out[at:, 3][live]).any() or dtype == F32
+            assert torch.isfinite(st[0, 0, [i for i in range(D + 1) if i != 3]]).all() and torch.isfinite(st[0, 1]).all()
+        v[at, 3] = old
+    assert ops.take_la_decay_device_status() == 0
+
+
+@pytest.mark.gpu
 def test_zero_features_give_zero_outputs():
     B, N, H, D = 1, 90, 2, 48
     q, k, v, ld, _ = make(B, N, H, D, BF16)
