@@ -313,17 +313,11 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       }
       volatile int* bad = bad_flag + c % T::BADS;
       const int* from = bad_from + c % T::BADS * D;
-      const bool poisoned = *bad != 0;  // the same for the four warps: cleared behind their common barrier
+      const bool poisoned = OUT && *bad != 0;  // the same for the four warps: cleared behind their common barrier
       if (poisoned) {
 #pragma unroll
         for (int i = 0; i < NS; ++i)
           if (held(i) && row_of(i) < D && from[row_of(i)] < C) S[i] = __uint_as_float(0x7fffffffu);
-        if (!OUT) {
-          asm volatile("bar.sync 2, 128;" ::: "memory");
-          for (int i = tid; i < D; i += 128) bad_from[c % T::BADS * D + i] = C;
-          if (tid == 0) *bad = 0;
-          __threadfence_block();
-        }
       }
       tcgen05_fence_before();
       __syncwarp();
@@ -476,6 +470,15 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     unsigned char* qrow = smem + T::OFF_Q + row * 128;
     unsigned char* vrow = smem + T::OFF_V + row * 128;
     auto piece = [&](int ch) -> uint32_t { return (uint32_t)((ch >> 3) * LT_BLK + (((ch & 7) ^ (row & 7)) << 4)); };
+    // Outputs must not see an infinity or NaN in v before its token (below).  Where a first launch has summed the segment, one
+    // key channel of that sum tells whether there is any; the sum itself is right to be NaN.
+    bool look = OUT;
+    if (OUT && a.npart > 0) {
+      const float* src = a.partial + (((int64_t)b * a.npart + seg) * a.H + h) * per;
+      bool odd = false;
+      for (int i = lane; i < D; i += 32) odd |= !(fabsf(__ldg(src + i * D)) <= 3.402823466e38f);
+      look = __any_sync(0xffffffffu, odd);
+    }
     auto relu4 = [&](uint4 r) { return make_uint4(ld_relu2(r.x), ld_relu2(r.y), ld_relu2(r.z), ld_relu2(r.w)); };
     auto publish = [&](uint32_t full) {
       fence_proxy_async_smem();
@@ -544,6 +547,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       // An infinity or NaN in v would meet the zero scores of the tokens before it: it is taken out here, and the state and
       // output warps put NaN where it belongs, from its token on.
       uint32_t big = 0u;
+      if (look)
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(i * PARTS + part));
