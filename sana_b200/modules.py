@@ -52,13 +52,32 @@ def _fp4_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.NvFp4Tens
     return entry[1]
 
 
+def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor":
+    """The 8-bit image of a projection weight (a scale for each 128 x 128 block), quantised once and kept on the module
+    until the parameter is modified or moved."""
+    cache = owner.__dict__.setdefault("_fp8_weights", {})
+    tag = (w2d.data_ptr(), w2d._version, tuple(w2d.shape))
+    entry = cache.get(key)
+    if entry is None or entry[0] != tag:
+        entry = (tag, ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK))
+        cache[key] = entry
+    return entry[1]
+
+
 def _project(owner: nn.Module, key: str, x2d, w2d: torch.Tensor, **epilogue) -> torch.Tensor:
     """``x2d @ w2d.T`` with the fused epilogue of :func:`ops.gemm`.  When ``owner.nvfp4`` is set
     both operands are NVFP4: the weight through :func:`_fp4_weight`; the activation is either
     already quantised by the kernel that produced it (an ``ops.NvFp4Tensor``) or quantised here,
-    with a measuring pass, on every call."""
+    with a measuring pass, on every call.  When ``owner.fp8`` is set both are E4M3 with a scale for
+    each block of 128 (:func:`ops.fp8_quantize`; no measuring pass)."""
     if isinstance(x2d, ops.NvFp4Tensor):
         return ops.gemm_nvfp4(x2d, _fp4_weight(owner, key, w2d), **epilogue)
+    if getattr(owner, "fp8", False):
+        if getattr(owner, "nvfp4", False):
+            raise ValueError("a projection is either NVFP4 or FP8: both flags are set")
+        if x2d.dtype != torch.bfloat16:
+            raise NotImplementedError("FP8 projections take bf16 activations and weights")
+        return ops.gemm_fp8(ops.fp8_quantize(x2d), _fp8_weight(owner, key, w2d), **epilogue)
     if not getattr(owner, "nvfp4", False):
         return ops.gemm(x2d, w2d, **epilogue)
     if x2d.dtype != torch.bfloat16:
@@ -121,6 +140,7 @@ class LiteLA(nn.Module):
             self.k_norm = nn.Identity()
         self.seq_shard: Optional[SequenceShard] = None
         self.nvfp4 = False  # quantise the qkv / proj projections to NVFP4
+        self.fp8 = False    # or to E4M3 with a scale for each block of 128
 
     # -- pieces shared with the fused block path --------------------------------------------
     def _core(self, qkv: torch.Tensor, B: int, N: int, rotary_emb=None, fp4_buf=None):
@@ -379,6 +399,64 @@ class CachedCausalAttention(LiteLAReLURope):
         return (out, kv_cache) if kv_cache is not None else out
 
 
+class DecayCausalAttention(nn.Module):
+    """Token-causal linear attention that forgets: ``S_t = exp(log_decay_h) S_{t-1} + [v_t; 1] phi(k_t)^T`` for each head,
+    outputs ``S_t[:D] phi(q_t) / (S_t[D] . phi(q_t) + eps)`` with ReLU features (``normalize=True``, the form of
+    :class:`LiteLA`) or ``D**-0.5 S_t[:D] q_t`` without.  With ``log_decay = 0`` the last token's state is LiteLA's.  No
+    counterpart upstream, whose causal attention works on whole chunks of frames and keeps everything.
+
+    ``forward`` takes a prompt, ``step`` one token of each sequence; the state passed between them is fp32
+    [B, heads, D+1, D] (row D = the key sum) whatever the dtype.  ``kv_heads`` < ``heads`` shares keys and values between
+    neighbouring query heads.  ``log_decay`` [heads] stays fp32 when the module is cast."""
+
+    def __init__(self, in_dim: int, out_dim: int, heads: int, kv_heads: Optional[int] = None, eps: float = 1e-8,
+                 normalize: bool = True, use_bias: bool = False):
+        super().__init__()
+        kv_heads = kv_heads or heads
+        D = out_dim // heads
+        if out_dim % heads or heads % kv_heads or D % 16 or not 16 <= D <= 128:
+            raise NotImplementedError("the kernels need out_dim / heads a multiple of 16 in [16, 128] and heads a multiple "
+                                      "of kv_heads")
+        self.in_dim, self.out_dim, self.heads, self.kv_heads, self.dim = in_dim, out_dim, heads, kv_heads, D
+        self.eps, self.normalize = eps, normalize
+        self.qkv = nn.Linear(in_dim, (heads + 2 * kv_heads) * D, bias=use_bias)
+        self.proj = nn.Linear(out_dim, out_dim)
+        # memories from two tokens to about a thousand, evenly on a logarithmic scale
+        self.log_decay = nn.Parameter(-torch.exp2(-1 - 9 * torch.arange(heads) / max(1, heads - 1)), requires_grad=False)
+        self.fp8 = False  # quantise both projections to E4M3 with a scale for each block of 128
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = self.log_decay.data
+        super()._apply(fn, *args, **kwargs)
+        self.log_decay.data = kept.to(device=self.log_decay.device, dtype=torch.float32)
+        return self
+
+    def _split(self, x2d: torch.Tensor):
+        qkv = _project(self, "qkv", x2d, self.qkv.weight, bias=self.qkv.bias)
+        a, b = self.heads * self.dim, (self.heads + self.kv_heads) * self.dim
+        return qkv[:, :a], qkv[:, a:b], qkv[:, b:]
+
+    def _form(self) -> dict:
+        return dict(relu=True, eps=float(self.eps)) if self.normalize else dict(scale=self.dim ** -0.5)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None):
+        """x [B, N, in_dim], optionally on top of ``state`` and with int32 ``lengths`` [B] of a padded batch (rows behind a
+        sequence give the projection's bias).  Returns (y [B, N, out_dim], state after the last token)."""
+        B, N, _ = x.shape
+        q, k, v = self._split(_as2d(x))
+        o, state = ops.la_decay(q, k, v, self.log_decay, B, N, self.heads, self.dim, prior=state, lengths=lengths, **self._form())
+        return _project(self, "proj", o, self.proj.weight, bias=self.proj.bias).reshape(B, N, -1), state
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [B, in_dim], one token of each sequence; ``state`` [pool, heads, D+1, D] is updated in place, row b in entry
+        ``slots[b]`` (see :func:`ops.la_decay_step`).  Returns y [B, out_dim]."""
+        q, k, v = self._split(x)
+        o = ops.la_decay_step(q, k, v, self.log_decay, state, self.heads, self.dim, slots=slots, **self._form())
+        return _project(self, "proj", o, self.proj.weight, bias=self.proj.bias)
+
+
 class ConvLayer(nn.Module):
     """Parameter holder with upstream's ``conv`` / ``norm`` / ``act`` attributes
     (basic_modules.py:32-99) so checkpoints load unchanged; GLUMBConv reads the weights and
@@ -430,6 +508,7 @@ class GLUMBConv(nn.Module):
         self.in_features, self.hidden_features, self.out_feature = in_features, hidden_features, out_feature
         self.seq_shard: Optional[SequenceShard] = None
         self.nvfp4 = False  # quantise the two 1x1 projections to NVFP4
+        self.fp8 = False    # or to E4M3 with a scale for each block of 128
 
     def _expand(self, z2d: torch.Tensor) -> torch.Tensor:
         c = self.inverted_conv.conv
@@ -768,9 +847,19 @@ class SanaMSBlock(nn.Module):
         forward after enabling it, and any forward after :meth:`recalibrate_nvfp4`, measures."""
         self.attn.nvfp4 = enabled
         self.mlp.nvfp4 = enabled
+        if enabled:
+            self.attn.fp8 = self.mlp.fp8 = False
         self.__dict__["_fp4_delayed"] = bool(enabled and delayed_scaling)
         self.__dict__["_fp4_margin"] = float(margin)
         self.__dict__["_fp4_state"] = None  # records + buffers, built by the calibrating forward
+
+    def set_fp8(self, enabled: bool = True) -> None:
+        """Run the same four projections on the 8-bit tensor cores: E4M3 values with one power-of-two scale for each 128
+        elements of an activation row and each 128 x 128 block of a weight.  Activations are quantised by one pass each
+        (a block's scale needs only its own elements).  Replaces the NVFP4 setting."""
+        if enabled:
+            self.set_nvfp4(False)
+        self.attn.fp8 = self.mlp.fp8 = bool(enabled)
 
     def recalibrate_nvfp4(self) -> None:
         """The next forward measures the activation maxima again (delayed scaling)."""
@@ -979,6 +1068,10 @@ class BlockStack(nn.Module):
     def set_nvfp4(self, enabled: bool = True, delayed_scaling: bool = False, margin: float = 1.0) -> None:
         for b in self.blocks:
             b.set_nvfp4(enabled, delayed_scaling, margin)
+
+    def set_fp8(self, enabled: bool = True) -> None:
+        for b in self.blocks:
+            b.set_fp8(enabled)
 
     @torch.no_grad()
     def forward(self, x, y, t, mask=None, HW=None, **kwargs):

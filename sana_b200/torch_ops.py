@@ -19,6 +19,11 @@ dtypes without touching the GPU.
     torch.ops.sana_b200.nvfp4_quantize(x) -> (codes, scale_tiles, scales)
     torch.ops.sana_b200.gemm_nvfp4(a_codes, a_sf, a_scales, w_codes, w_sf, w_scales, bias, act, relu_cols,
                                    gate_table, gate_t, gate_row, rows_per_batch, residual)
+    torch.ops.sana_b200.fp8_quantize(x, block_rows) -> (codes, scales)
+    torch.ops.sana_b200.gemm_fp8(a_codes, a_scales, a_block_rows, w_codes, w_scales, w_block_rows, bias, act, relu_cols,
+                                 gate_table, gate_t, gate_row, rows_per_batch, residual)
+    torch.ops.sana_b200.la_decay(q, k, v, log_decay, B, N, H, D, scale, relu, eps, prior, lengths) -> (out, state)
+    torch.ops.sana_b200.la_decay_step(q, k, v, log_decay, state, H, D, scale, relu, eps, slots)  # state in place
 
 They are thin: each forwards to :mod:`sana_b200.ops`, which passes raw device pointers and the
 current stream to libsana_b200.so.  The modules call :mod:`sana_b200.ops` directly (same
@@ -36,7 +41,8 @@ _lib_ns = "sana_b200"
 # the ctypes-level functions, captured before any routing replaces the names in `ops`
 _D = {n: getattr(ops, n) for n in ("gemm", "ln_modulate", "ln_modulate_rows", "la_state", "la_apply", "dwconv_glu", "rmsnorm_",
                                    "rope_", "cross_attention", "la_rope_state", "la_rope_apply", "add_f32", "patchify",
-                                   "unpatchify", "timestep_embedding", "silu", "nvfp4_quantize", "gemm_nvfp4")}
+                                   "unpatchify", "timestep_embedding", "silu", "nvfp4_quantize", "gemm_nvfp4",
+                                   "fp8_quantize", "gemm_fp8", "la_decay", "la_decay_step")}
 
 
 @torch.library.custom_op(f"{_lib_ns}::gemm", mutates_args=())
@@ -244,6 +250,62 @@ def _(a_codes, a_sf, a_scales, w_codes, w_sf, w_scales, bias, act, relu_cols, ga
     return a_codes.new_empty(a_codes.shape[0], w_codes.shape[0], dtype=torch.bfloat16)
 
 
+def _fp8_scales(rows: int, K: int, block_rows: int) -> Tuple[int, int]:
+    return (rows + block_rows - 1) // block_rows, (K + 127) // 128
+
+
+@torch.library.custom_op(f"{_lib_ns}::fp8_quantize", mutates_args=())
+def fp8_quantize(x: torch.Tensor, block_rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    t = _D["fp8_quantize"](x, block_rows)
+    return t.q, t.scales
+
+
+@fp8_quantize.register_fake
+def _(x, block_rows):
+    R, kb = _fp8_scales(x.shape[0], x.shape[1], block_rows)
+    # rows of scales are padded to whole words of four
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(R, (kb + 3) // 4 * 4, dtype=torch.uint8)[:, :kb]
+
+
+@torch.library.custom_op(f"{_lib_ns}::gemm_fp8", mutates_args=())
+def gemm_fp8(a_codes: torch.Tensor, a_scales: torch.Tensor, a_block_rows: int, w_codes: torch.Tensor, w_scales: torch.Tensor,
+             w_block_rows: int, bias: Optional[torch.Tensor], act: int, relu_cols: int, gate_table: Optional[torch.Tensor],
+             gate_t: Optional[torch.Tensor], gate_row: int, rows_per_batch: int,
+             residual: Optional[torch.Tensor]) -> torch.Tensor:
+    a, w = ops.Fp8Tensor(a_codes, a_scales, a_block_rows), ops.Fp8Tensor(w_codes, w_scales, w_block_rows)
+    gate = (gate_table, gate_t, gate_row, rows_per_batch) if gate_table is not None else None
+    return _D["gemm_fp8"](a, w, bias=bias, act=act, relu_cols=relu_cols, gate=gate, residual=residual)
+
+
+@gemm_fp8.register_fake
+def _(a_codes, a_scales, a_block_rows, w_codes, w_scales, w_block_rows, bias, act, relu_cols, gate_table, gate_t, gate_row,
+      rows_per_batch, residual):
+    return a_codes.new_empty(a_codes.shape[0], w_codes.shape[0], dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_lib_ns}::la_decay", mutates_args=())
+def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, B: int, N: int, H: int, D: int,
+             scale: float, relu: bool, eps: Optional[float], prior: Optional[torch.Tensor],
+             lengths: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _D["la_decay"](q, k, v, log_decay, B, N, H, D, scale, relu, eps, prior, lengths)
+
+
+@la_decay.register_fake
+def _(q, k, v, log_decay, B, N, H, D, scale, relu, eps, prior, lengths):
+    return q.new_empty(B * N, H * D), q.new_empty(B, H, D + 1, D, dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_lib_ns}::la_decay_step", mutates_args=("state",))
+def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, H: int,
+                  D: int, scale: float, relu: bool, eps: Optional[float], slots: Optional[torch.Tensor]) -> torch.Tensor:
+    return _D["la_decay_step"](q, k, v, log_decay, state, H, D, scale, relu, eps, slots)
+
+
+@la_decay_step.register_fake
+def _(q, k, v, log_decay, state, H, D, scale, relu, eps, slots):
+    return q.new_empty(q.shape[0], H * D)
+
+
 # ---- optional: the modules through the dispatcher ---------------------------------------------------------
 # The modules call `sana_b200.ops` directly (no dispatcher overhead per launch).  For tracing, export or fake-tensor
 # shape propagation of a whole module, route_modules(True) replaces those names in `ops` by wrappers that go
@@ -301,12 +363,25 @@ def _r_timestep_embedding(t, dim, dtype, max_period=10000.0):
     return torch.ops.sana_b200.timestep_embedding(t, dim, dtype, float(max_period))
 
 
+def _r_la_decay(q, k, v, log_decay, B, N, H, D, scale=1.0, relu=False, eps=None, prior=None, lengths=None, out=None):
+    if out is not None:
+        return _D["la_decay"](q, k, v, log_decay, B, N, H, D, scale, relu, eps, prior, lengths, out)
+    return torch.ops.sana_b200.la_decay(q, k, v, log_decay, B, N, H, D, float(scale), relu, eps, prior, lengths)
+
+
+def _r_la_decay_step(q, k, v, log_decay, state, H, D, scale=1.0, relu=False, eps=None, slots=None, out=None):
+    if out is not None:
+        return _D["la_decay_step"](q, k, v, log_decay, state, H, D, scale, relu, eps, slots, out)
+    return torch.ops.sana_b200.la_decay_step(q, k, v, log_decay, state, H, D, float(scale), relu, eps, slots)
+
+
 _ROUTED = {"gemm": _r_gemm, "ln_modulate": _r_ln_modulate, "la_state": torch.ops.sana_b200.la_state, "la_apply": _r_la_apply,
            "dwconv_glu": _r_dwconv_glu, "rmsnorm_": _r_rmsnorm_, "rope_": _r_rope_,
            "cross_attention": torch.ops.sana_b200.cross_attention, "la_rope_state": _r_la_rope_state,
            "la_rope_apply": _r_la_rope_apply, "add_f32": torch.ops.sana_b200.add_f32, "ln_modulate_rows": _r_ln_modulate_rows,
            "patchify": torch.ops.sana_b200.patchify, "unpatchify": torch.ops.sana_b200.unpatchify,
-           "timestep_embedding": _r_timestep_embedding, "silu": torch.ops.sana_b200.silu}
+           "timestep_embedding": _r_timestep_embedding, "silu": torch.ops.sana_b200.silu, "la_decay": _r_la_decay,
+           "la_decay_step": _r_la_decay_step}
 
 
 def route_modules(enabled: bool = True) -> None:
