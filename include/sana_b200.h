@@ -253,8 +253,8 @@ int sana_la_rope_take_device_status(int* status_out);
  *   multiple of Hk (query head h reads key/value head h / (H / Hk)); D a multiple of 16 in [16, 128]; rows 16-byte aligned
  *   log_decay [H] fp32;  prior [B, H, D+1, D] fp32 (the state before the first token) or NULL;  state: the state after
  *   the last token, a buffer other than prior
- *   lengths [B] int32 on the device, or NULL: sequence b has lengths[b] tokens (clamped to [0, N]); the rows behind them
- *   are not read, their outputs are zeros, and the state is the one after token lengths[b] - 1 (or prior, or zeros)
+ *   lengths [B] int32 on the device, or NULL: sequence b has lengths[b] tokens (clamped to [0, N]); what the
+ *   rows behind them hold has no effect, their outputs are zeros, and the state is the one after token lengths[b] - 1 (or prior, or zeros)
  *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
  *   arguments), 16-byte aligned.
  * State, decays and normalisers are fp32; bf16: both sides of the products are bf16, the state enters the product with q
@@ -453,7 +453,8 @@ int sana_dwconv_glu_amax(const void* u, const void* halo_top, const void* halo_b
  *   A @ W^T = sum over blocks of 2^(ea + ew) * (product of the codes), fp32 accumulation.  K % 16 == 0, N % 8 == 0.
  *   Scale rows must be 4-byte aligned, ldsfa / ldsfw multiples of 4, and each row readable up to the next multiple
  *   of 4 blocks (what lies there is not used).  tcgen05.mma kind::mxf8f6f4, which applies the scales itself;
- *   M >= 2048: CTA pairs on 256 x 256 tiles, else one CTA on 128 x 128 tiles (sana_gemm_set_variant overrides).
+ *   M >= 2048: CTA pairs on 256 x 256 tiles, else one CTA on 128 x 128 tiles; M <= 16: the weight is streamed once and
+ *   multiplied warp by warp (sana_gemm_set_variant overrides).
  */
 int sana_fp8_quantize(const void* x, int64_t ld, void* q, void* sf, int64_t ldsf, int64_t rows, int64_t K,
                       int block_rows, int dtype, void* stream);

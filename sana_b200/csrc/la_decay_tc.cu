@@ -20,6 +20,15 @@
 // it only serves the outputs (2^-16, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
 // rows of one product, and the state warps add them; an instruction costs 42 + N / 2 cycles whatever part of its rows
 // is used.  All waits are bounded.
+//
+// Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
+// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 229-240 us (2.5 TB/s; 90); 4 x up to 4096, 16 heads of
+// 64 over 8 of k and v 91-95.  What
+// bounds it is the length of a chunk's chain - copy, transform, products, join, state operand, products, output, each behind
+// a barrier and with one warp per scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.
+// Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per SM overlap theirs; wide heads
+// fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles that poll several barriers in
+// turn were tried and were slower.
 #include "la_decay.cuh"
 
 namespace sana {
@@ -107,8 +116,6 @@ __device__ __forceinline__ uint32_t lt_ld1(uint32_t taddr) {
   return r;
 }
 
-// Bounded wait like mbar_wait, by all lanes of a warp and with the plain poll: the suspend hint of mbar_wait puts the warp
-// to sleep in steps, up to a microsecond past the arrival, and a chunk passes through eight waits in a row.
 // whether a phase is complete, without waiting
 __device__ __forceinline__ bool lt_test(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -116,6 +123,8 @@ __device__ __forceinline__ bool lt_test(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
+// Bounded wait like mbar_wait, by all lanes of a warp and with the plain poll: the suspend hint of mbar_wait puts the warp
+// to sleep in steps, up to a microsecond past the arrival, and a chunk passes through eight waits in a row.
 __device__ __forceinline__ bool lt_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait_poll(bar, parity))) return true;
   const long long t0 = clock64();
@@ -547,11 +556,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       // An infinity or NaN in v would meet the zero scores of the tokens before it: it is taken out here, and the state and
       // output warps put NaN where it belongs, from its token on.
       uint32_t big = 0u;
-      if (look)
+      if (look) {
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(i * PARTS + part));
-        big = __vmaxu2(big, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        for (int i = 0; i < PIECES; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vt + piece(i * PARTS + part));
+          big = __vmaxu2(big, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        }
       }
       if (live && max(big & 0xffffu, big >> 16) >= 0x7f80u) {
 #pragma unroll 1
