@@ -103,6 +103,11 @@ __device__ __forceinline__ void lt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Nothing that uses these registers may move above the wait for the loads that fill them, while others are under way.
+__device__ __forceinline__ void lt_arrived(uint32_t (&r)[16]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+               "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
 __device__ __forceinline__ void lt_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -314,6 +319,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
         for (int g = 0; g < D / 16; ++g) {
           tmem_ld_wait();
+          lt_arrived(d[g & 1]);
           if (g + 1 < D / 16) tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * (g + 1)), d[(g + 1) & 1]);
 #pragma unroll
           for (int e = 0; e < 16; ++e) S[16 * g + e] = fmaf(whole, S[16 * g + e], __uint_as_float(d[g & 1][e]));
@@ -383,6 +389,8 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
           }
           tmem_ld_wait();
+          lt_arrived(x);
+          lt_arrived(y);
         }
         if (poisoned) {
           asm volatile("bar.sync 2, 128;" ::: "memory");
@@ -523,8 +531,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         publish(qfull);
       } else {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kempty);
+        publish(kempty);  // the fence holds back the hand-over until the loads are done: without ReLU nothing else has waited for them
       }
       if (!lt_wait(wempty + wbar, ph ^ 1u, abort_flag, 6)) break;
       const float wt = live ? pow_s[nv - 1 - row] : 0.f;

@@ -119,6 +119,35 @@ def test_long_sequences_in_segments(dtype, D, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D", [(4, 4096, 16, 8, 64), (4, 4096, 16, 16, 48), (2, 8192, 20, 20, 32), (8, 2048, 20, 20, 112)])
+def test_many_segments_give_the_same_bits_every_time(B, N, H, Hk, D, relu):
+    """More segments than multiprocessors, slow decays (nothing that goes wrong on the way is forgotten), and the chunks of
+    a segment against single tokens: the state of a few heads in 64 bits."""
+    q, k, v, _, p = make(B, N, H, D, BF16, Hk, prior=True, relu=relu)
+    ld = -torch.exp2(-torch.linspace(4, 14, H)).cuda()
+    lengths = torch.tensor([N - 77 * b for b in range(B)], dtype=torch.int32).cuda()
+    kw = dict(relu=relu, eps=1e-8 if relu else None, prior=p)
+    for n in (lengths, None):
+        out, st = ops.la_decay(q, k, v, ld, B, N, H, D, lengths=n, **kw)
+        for _ in range(8):
+            o2, s2 = ops.la_decay(q, k, v, ld, B, N, H, D, lengths=n, **kw)
+            assert torch.equal(o2, out) and torch.equal(s2, st)
+        for b in (0, B - 1):
+            m = int(lengths[b]) if n is not None else N
+            for h in (0, H // 2, H - 1):
+                hk = h // (H // Hk)
+                rows = slice(b * N, b * N + m)
+                f = k[rows, hk * D:(hk + 1) * D].double()
+                f = f.clamp(min=0) if relu else f
+                v1 = torch.cat([v[rows, hk * D:(hk + 1) * D].double(), torch.ones(m, 1, dtype=torch.float64, device="cuda")], 1)
+                w = torch.exp(ld[h].double() * torch.arange(m - 1, -1, -1, device="cuda"))[:, None]
+                whole = torch.exp(ld[h].double() * m)
+                want, mag = v1.T @ (w * f) + whole * p[b, h].double(), v1.abs().T @ (w * f.abs()) + whole * p[b, h].double().abs()
+                close(st[b, h], want.cpu(), mag.cpu(), F32, (b, h), state_tol(N, BF16))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [32, 112])
 def test_decays_from_none_to_total(dtype, D):
