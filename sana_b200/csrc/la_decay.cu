@@ -643,11 +643,11 @@ constexpr int64_t LD_TC_TOKENS = LD_C + 1;  // shortest sequences the tcgen05 ke
 // the heads alone leave the GPU partly empty, since every cut re-reads k and v.  Cost of a choice = waves x (tokens of a
 // segment, plus half as many again for the first launch, plus about two chunks for reading the states before it).
 template <int D>
-static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, int* nseg, int* npart) {
+static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, bool ragged, int* seg_len, int* nseg, int* npart) {
   if (dtype == SANA_BF16) {
     LdPlan p = {LD_C, 1};
     *npart = 0;
-    if (N >= LD_TC_TOKENS) p = ld_tc_plan(B, N, H, D, npart);
+    if (N >= LD_TC_TOKENS) p = ld_tc_plan(B, N, H, D, ragged, npart);
     *seg_len = p.seg_len, *nseg = p.nseg;
     return;
   }
@@ -666,7 +666,7 @@ static void ld_plan(int64_t B, int64_t N, int64_t H, int dtype, int* seg_len, in
 
 template <int D>
 static int launch_decay(LdArgs& a, int64_t B, int dtype, int64_t workspace_bytes, cudaStream_t st) {
-  ld_plan<D>(B, a.N, a.H, dtype, &a.seg_len, &a.nseg, &a.npart);
+  ld_plan<D>(B, a.N, a.H, dtype, a.lengths != nullptr, &a.seg_len, &a.nseg, &a.npart);
   SANA_REQUIRE(workspace_bytes >= (int64_t)4 * B * a.npart * a.H * (D + 1) * D, "sana_la_decay: workspace too small");
   if (dtype == SANA_BF16) {
     if (a.N >= LD_TC_TOKENS) return launch_decay_tc(a, B, D, st);
@@ -730,9 +730,9 @@ using namespace sana;
 
 extern "C" int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype) {
   if (B <= 0 || N <= 0 || N >= ((int64_t)1 << 30) || H <= 0 || !ld_head_dim(D) || (dtype != SANA_BF16 && dtype != SANA_F32)) return -1;
-  int len = 0, nseg = 1, npart = 0;
-  LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, &len, &nseg, &npart)));
-  return (int64_t)4 * B * npart * H * (D + 1) * D;
+  int len = 0, nseg = 1, npart[2] = {0, 0};
+  for (int ragged = 0; ragged < 2; ++ragged) LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, ragged != 0, &len, &nseg, &npart[ragged])));
+  return (int64_t)4 * B * (npart[0] > npart[1] ? npart[0] : npart[1]) * H * (D + 1) * D;
 }
 
 extern "C" int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* log_decay,

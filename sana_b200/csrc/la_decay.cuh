@@ -43,7 +43,7 @@ struct LdPlan {
 };
 
 // tcgen05 kernels (la_decay_tc.cu); D a multiple of 16 in [16, 128]
-LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, int* npart);
+LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, bool ragged, int* npart);  // ragged: lengths are given
 int launch_decay_tc(LdArgs& a, int64_t B, int64_t D, cudaStream_t st);
 
 }  // namespace sana

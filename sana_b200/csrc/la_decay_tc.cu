@@ -231,7 +231,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     float S[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) S[i] = 0.f;
-    if (OUT && sin) {  // the state before this segment
+    if (OUT && sin && (chunks > 0 || seg == a.nseg - 1)) {  // the state before this segment
       auto add = [&](const float* src, float f) {
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -776,14 +776,33 @@ static int lt_run(const LdArgs& a, int64_t B, cudaStream_t st) {
   return lt_launch<D, 2, true>(m, a, a.nseg, B, st);
 }
 
-LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, int* npart) {
+// Cost of a split = waves of CTAs x the time of a segment.  A padded batch is taken to hold lengths spread evenly over
+// [0, N]: CTAs behind the end of a sequence leave at once, (segments + 1) / 2 of a sequence's have work, and these fill one
+// another's gaps, so the waves are not rounded up.  Its split replaces the first one only where it promises at least 15 %,
+// since sequences that all reach N lose by it: 4 x 4096, 16 heads of 64, four segments against two, lengths spread 68 us
+// against 94, one long sequence 57 against 94, all full 109 against 96.
+LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, bool ragged, int* npart) {
   const int64_t units = B * H, slots = (int64_t)sm_count() * (D <= 32 ? 2 : 1), chunks = ceil_div(N, LT_C);
+  auto segment = [&](int64_t len, int64_t real) -> int64_t {  // tenths of a chunk
+    return real > 1 || D == 128 ? 16 * len + 20 + 2 * real : 12 * len + 10;
+  };
+  auto spread = [&](int64_t len, int64_t real) -> double {
+    const double waves = 0.5 * (double)(units * (real + 1)) / (double)slots;
+    return (waves > 1. ? waves : 1.) * (double)segment(len, real);
+  };
   int64_t best = -1, best_len = chunks;
   for (int64_t n = 1; n <= chunks && n <= 64; ++n) {
-    const int64_t len = ceil_div(chunks, n), real = ceil_div(chunks, len), waves = ceil_div(units * real, slots);
-    const bool two = real > 1 || D == 128;
-    const int64_t cost = waves * (two ? 16 * len + 20 + 2 * real : 12 * len + 10);  // tenths of a chunk
+    const int64_t len = ceil_div(chunks, n), real = ceil_div(chunks, len);
+    const int64_t cost = ceil_div(units * real, slots) * segment(len, real);
     if (best < 0 || cost < best) best = cost, best_len = len;
+  }
+  if (ragged && B > 1) {
+    double limit = 0.85 * spread(best_len, ceil_div(chunks, best_len));
+    for (int64_t n = 1; n <= chunks && n <= 64; ++n) {
+      const int64_t len = ceil_div(chunks, n);
+      const double cost = spread(len, ceil_div(chunks, len));
+      if (cost < limit) limit = cost, best_len = len;
+    }
   }
   LdPlan p;
   p.seg_len = (int)(best_len * LT_C);
