@@ -258,7 +258,7 @@ int sana_la_rope_take_device_status(int* status_out);
  *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
  *   arguments), 16-byte aligned.
  * State, decays and normalisers are fp32; bf16: both sides of the products are bf16, the state enters the product with q
- * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once.  Bit-reproducible.  An infinity or
+ * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once (64 tokens or fewer: two terms).  Bit-reproducible.  An infinity or
  * NaN in v gives NaN in its channel from its token on, one in k or q what the sums make of it; no output before the
  * token is touched.
  *

@@ -19,8 +19,9 @@
 // fragment of v that multiplies the scores is the A operand of the state update, so the state never moves and v is read
 // from shared memory once.
 // The state stays within a few 2^-24 of fp32: the weighted v is split into three bf16 terms (8 bits each) before the
-// tensor core sees it.  In S phi(q) the state enters as two bf16 terms (2^-16); the scores are rounded to bf16 once,
-// like the output.  The normaliser is summed in fp32 from the unrounded scores.
+// tensor core sees it.  In S phi(q) the state, and before v the scores, enter as two bf16 terms (2^-16): an output of a few
+// tokens would feel one rounding of a score as much as its own (a longer sum averages them: la_decay_tc.cu rounds once).
+// The normaliser is summed in fp32 from the unrounded scores.
 // fp32: the chunked form on the CUDA cores.  A sequence is split over CTAs into segments when there are fewer heads than the
 // GPU has room for: a first launch computes what each segment adds to the state, and each CTA of the second combines those
 // of the segments before its own, in order (nothing depends on the order in which CTAs run).
@@ -57,7 +58,7 @@ struct Ld {
   static constexpr int TILE = LD_C * ROW;
   static constexpr int PROW = 2 * LD_C + 16;               // scores; the 16 spare bytes hold the four partial row sums
   static constexpr int OFF_P = 3 * TILE;                   // q, k, v | scores | powers | key sum | q . key sum |
-  static constexpr int OFF_POW = OFF_P + LD_C * PROW;
+  static constexpr int OFF_POW = OFF_P + 2 * LD_C * PROW;  // two bf16 terms of the scores
   static constexpr int OFF_Z = OFF_POW + 4 * (LD_C + 4);
   static constexpr int OFF_QZ = OFF_Z + 4 * D;
   static constexpr int OFF_BAD = OFF_QZ + 4 * LD_C;         // first token whose v is not finite, by channel
@@ -203,8 +204,11 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_short_kernel(const Ld
             unsigned char* pr = smem + T::OFF_P + (16 * mi + g) * T::PROW;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              *reinterpret_cast<uint32_t*>(pr + 2 * (16 * ni + 8 * n + c2)) = pack_bf16(p[n][0], p[n][1]);
-              *reinterpret_cast<uint32_t*>(pr + 8 * T::PROW + 2 * (16 * ni + 8 * n + c2)) = pack_bf16(p[n][2], p[n][3]);
+              unsigned char* at = pr + 2 * (16 * ni + 8 * n + c2);
+              *reinterpret_cast<uint32_t*>(at) = ld_split(p[n][0], p[n][1]);
+              *reinterpret_cast<uint32_t*>(at + 8 * T::PROW) = ld_split(p[n][2], p[n][3]);
+              *reinterpret_cast<uint32_t*>(at + C * T::PROW) = pack_bf16(p[n][0], p[n][1]);
+              *reinterpret_cast<uint32_t*>(at + (C + 8) * T::PROW) = pack_bf16(p[n][2], p[n][3]);
             }
             if (a.normalise) {
 #pragma unroll
@@ -280,9 +284,12 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_short_kernel(const Ld
 #pragma unroll
         for (int kt = 0; kt <= mi; ++kt) {
           uint32_t pa[4];
-          ldsm_x4(pa, Ps + (16 * mi + (lane & 15)) * T::PROW + (lane >> 4) * 16 + kt * 32);
-          mma_bf16_16816(o[mi][0], pa[0], pa[1], pa[2], pa[3], vf[kt][0], vf[kt][1]);
-          mma_bf16_16816(o[mi][1], pa[0], pa[1], pa[2], pa[3], vf[kt][2], vf[kt][3]);
+#pragma unroll
+          for (int s = 1; s >= 0; --s) {  // the second terms first
+            ldsm_x4(pa, Ps + (s * C + 16 * mi + (lane & 15)) * T::PROW + (lane >> 4) * 16 + kt * 32);
+            mma_bf16_16816(o[mi][0], pa[0], pa[1], pa[2], pa[3], vf[kt][0], vf[kt][1]);
+            mma_bf16_16816(o[mi][1], pa[0], pa[1], pa[2], pa[3], vf[kt][2], vf[kt][3]);
+          }
         }
         float m0 = a.scale, m1 = a.scale;
         if (a.normalise) {

@@ -16,15 +16,15 @@
 // sum to it (S = lambda^C S + dS: one rounded multiply-add per chunk, since the tensor core truncates its sums), write it
 // as the bf16 operand of O1, and finish the outputs; warps 4-7 decay and mask the scores; the next 4 or 8 warps weight the
 // keys, apply ReLU in place and put the ones column back beside v; one warp issues the products, one the copies.
-// The weighted k is split into NT bf16 terms: 3 where the state that leaves the kernel is exact to fp32 (2^-24), 2 where
-// it only serves the outputs (2^-16, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
+// The weighted k is split into NT bf16 terms: 3 where the state leaves the kernel (2^-24; the truncation of a chunk's 24
+// products adds up to 2e-6 where everything has one sign and nothing decays, 3e-7 otherwise), 2 where it only serves the
+// outputs (2^-16, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
 // rows of one product, and the state warps add them; an instruction costs 42 + N / 2 cycles whatever part of its rows
 // is used.  All waits are bounded.
 //
 // Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
-// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 229-240 us (2.5 TB/s; 90); 4 x up to 4096, 16 heads of
-// 64 over 8 of k and v 91-95.  What
-// bounds it is the length of a chunk's chain - copy, transform, products, join, state operand, products, output, each behind
+// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 229-240 us (2.5 TB/s; 90); 4 x up to 4096, 16 heads of 64 over 8
+// of k and v 68-91.  What bounds it is the length of a chunk's chain - copy, transform, products, join, state operand, products, output, each behind
 // a barrier and with one warp per scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.
 // Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per SM overlap theirs; wide heads
 // fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles that poll several barriers in
