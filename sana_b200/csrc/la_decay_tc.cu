@@ -24,11 +24,11 @@
 //
 // Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
 // rate would allow 45); 8 x 4096 tokens, 70 heads of 32 229-240 us (2.5 TB/s; 90); 4 x up to 4096, 16 heads of 64 over 8
-// of k and v 68-91.  What bounds it is the length of a chunk's chain - copy, transform, products, join, state operand, products, output, each behind
-// a barrier and with one warp per scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.
-// Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per SM overlap theirs; wide heads
-// fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles that poll several barriers in
-// turn were tried and were slower.
+// of k and v 68-91.  What bounds it is the length of a chunk's chain - copy, transform, products, join, state operand,
+// products, output, each behind a barrier and with one warp per scheduler for each role: the tensor pipe is busy 17-22 % of
+// the time and DRAM 25-38 %.  Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per
+// SM overlap theirs; wide heads fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles
+// that poll several barriers in turn were tried and were slower.
 #include "la_decay.cuh"
 
 namespace sana {
