@@ -662,10 +662,10 @@ __device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint3
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// d * 2^(s - 254), s the sum of two E8M0 bytes: in two factors, so that neither leaves the range of fp32
-__device__ __forceinline__ float f8_scaled(float d, int s) {
-  const int h = s >> 1;
-  return d * __uint_as_float((uint32_t)h << 23) * __uint_as_float((uint32_t)(s - h) << 23);
+// d * 2^(e + f - 254), e and f E8M0 bytes (255: NaN): in two factors, so that neither leaves the range of fp32
+__device__ __forceinline__ float f8_scaled(float d, int e, int f) {
+  const int s = e + f, h = s >> 1;
+  return d * __uint_as_float(max(e, f) == 255 ? 0x7fffffffu : (uint32_t)h << 23) * __uint_as_float((uint32_t)(s - h) << 23);
 }
 
 template <int NT8, int WARPS>
@@ -702,10 +702,10 @@ __global__ void __launch_bounds__(32 * WARPS) gemm_fp8_rows_kernel(const unsigne
       const int ma = 8 * t + 2 * c, mb = ma + 1;
       const int f0 = ma < args.M ? __ldg(args.sa.p + (ma >> args.sa.shift) * args.sa.ld + kb) : 127;
       const int f1 = mb < args.M ? __ldg(args.sa.p + (mb >> args.sa.shift) * args.sa.ld + kb) : 127;
-      acc[t][0] += f8_scaled(d[0], e0 + f0);
-      acc[t][1] += f8_scaled(d[1], e0 + f1);
-      acc[t][2] += f8_scaled(d[2], e1 + f0);
-      acc[t][3] += f8_scaled(d[3], e1 + f1);
+      acc[t][0] += f8_scaled(d[0], e0, f0);
+      acc[t][1] += f8_scaled(d[1], e0, f1);
+      acc[t][2] += f8_scaled(d[2], e1, f0);
+      acc[t][3] += f8_scaled(d[3], e1, f1);
     }
   }
 #pragma unroll

@@ -54,12 +54,20 @@ def _fp4_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.NvFp4Tens
 
 def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor":
     """The 8-bit image of a projection weight (a scale for each 128 x 128 block), quantised once and kept on the module
-    until the parameter is modified or moved."""
+    until the parameter is modified (other than through ``.data``, which leaves no trace), replaced or moved.  The entry
+    holds the weight's storage, so that no other weight can turn up at its address, and the host waits for the one
+    quantisation, so that every stream may use it.  Not kept, but made by every call: under a stream capture (the image would
+    exist from the first replay on) and for inference tensors (whose changes are not counted)."""
+    if w2d.is_inference():
+        return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
     cache = owner.__dict__.setdefault("_fp8_weights", {})
     tag = (w2d.data_ptr(), w2d._version, tuple(w2d.shape))
     entry = cache.get(key)
     if entry is None or entry[0] != tag:
-        entry = (tag, ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK))
+        entry = (tag, ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK), w2d.detach())
+        if torch.cuda.is_current_stream_capturing():
+            return entry[1]
+        torch.cuda.current_stream(w2d.device).synchronize()
         cache[key] = entry
     return entry[1]
 

@@ -749,7 +749,7 @@ def _device_of(what: str, *ts: Optional[torch.Tensor]) -> int:
 class Fp8Tensor:
     """A [rows, K] matrix as E4M3 codes ``q`` (float8_e4m3fn, contiguous) with one power-of-two scale for each block of
     ``block_rows`` rows x 128 columns: ``scales`` [ceil(rows / block_rows), ceil(K / 128)] uint8 holds exponent + 127
-    (E8M0).  Scale rows are read in words of four, so ``scales`` is copied here when its rows are not padded that far."""
+    (E8M0; 255 is NaN).  Scale rows are read in words of four, so ``scales`` is copied here when its rows are not padded that far."""
 
     __slots__ = ("q", "scales", "block_rows", "rows", "K")
 
@@ -784,7 +784,8 @@ class Fp8Tensor:
     def dequantize(self) -> torch.Tensor:
         """fp32 [rows, K] reconstruction (torch math; for tests and diagnostics only)."""
         e = self.scales.to(torch.int32).repeat_interleave(self.block_rows, 0)[:self.rows]
-        return torch.ldexp(self.q.float(), e.repeat_interleave(FP8_BLOCK, 1)[:, :self.K] - 127)
+        e = e.repeat_interleave(FP8_BLOCK, 1)[:, :self.K]
+        return torch.ldexp(self.q.float(), e - 127).masked_fill(e == 255, float("nan"))
 
 
 def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
@@ -880,7 +881,7 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
 
     q [B*N, H*D] and k, v [B*N, Hk*D] views (column blocks of a projection), H a multiple of Hk; log_decay fp32 [H], not
     positive; prior fp32 [B, H, D+1, D], the state carried in; lengths int32 [B] for a padded batch (rows behind a
-    sequence give zeros).  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
+    sequence give zeros); out must not overlap k or v.  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
     dev = _device_of("la_decay", q, k, v, log_decay, prior, lengths, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -904,7 +905,8 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
         raise SanaLibraryError("la_decay: sizes out of range")
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _lib.check(lib.sana_la_decay(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
-                                 prior.data_ptr() if prior is not None else None, lens, state.data_ptr(), out.data_ptr(), ldo,
+                                 prior.data_ptr() if prior is not None else None, lens, state.data_ptr(), out.data_ptr(),
+                                 ldo if ro > 1 else max(ldo, co),
                                  ws.data_ptr() if ws is not None else None, ws_bytes, B, N, H, Hk, D, scale, 1 if relu else 0,
                                  -1.0 if eps is None else eps, dt, _stream_of(dev)), "sana_la_decay")
     counters.launches += 2 if ws_bytes else 1
@@ -917,7 +919,7 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
     """One token of each of B sequences through :func:`la_decay`'s recurrence: q [B, H*D], k, v [B, Hk*D]; ``state`` fp32
     [pool, H, D+1, D] is updated in place, row b using entry ``slots[b]`` (int32 [B]; without it, entry b).  A slot of -1
     marks an unused row (output zeros); a slot outside the pool, or one an earlier row names already, gives NaN outputs
-    and leaves the state alone.  Returns out [B, H*D]."""
+    and leaves the state alone; out must not overlap k or v.  Returns out [B, H*D]."""
     dev = _device_of("la_decay_step", q, k, v, log_decay, state, slots, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):

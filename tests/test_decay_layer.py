@@ -100,6 +100,45 @@ def test_serving_batch_with_slots_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_the_kept_weight_image_is_that_of_the_weight():
+    m = layer()
+    m.fp8 = True
+    x = torch.randn(1, 70, 192).to(BF16).cuda()
+    y = m(x)[0]
+    for seed in (1, 2, 3):  # new weights of the same size, which the allocator would put where freed ones were
+        m.qkv.weight = None
+        m.qkv.weight = torch.nn.Parameter(layer(seed=seed).qkv.weight.detach().clone(), requires_grad=False)
+        kept, fresh = m(x)[0], layer()
+        fresh.load_state_dict(m.state_dict())
+        fresh.fp8 = True
+        assert torch.equal(kept, fresh(x)[0]) and not torch.equal(kept, y)
+    with torch.inference_mode():  # changes of inference tensors are not counted
+        n = layer()
+        n.fp8 = True
+        first = n(x)[0]
+        n.proj.weight.mul_(2)
+        assert not torch.equal(n(x)[0], first)
+
+
+@pytest.mark.gpu
+def test_a_capture_without_warm_up_keeps_nothing():
+    m = layer()
+    m.fp8 = True
+    x = torch.randn(1, 70, 192).to(BF16).cuda()
+    ops.gemm_fp8(ops.fp8_quantize(x[0]), ops.fp8_quantize(m.qkv.weight, 128))  # the library is loaded
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, st = m(x)
+    eager = m(x)  # before the first replay
+    g.replay()
+    assert torch.equal(y, eager[0]) and torch.equal(st, eager[1])
+    with torch.no_grad():
+        m.qkv.weight.mul_(0.5)
+    g.replay()
+    assert torch.equal(y, m(x)[0])
+
+
+@pytest.mark.gpu
 def test_block_with_8_bit_projections():
     """Every operand is off by at most 2^-4 of itself (rms 2^-4 / sqrt 3), so a projection by sqrt 2 of that in norm; four
     projections follow one another in the block, and their branches' share of the output is at most all of it."""

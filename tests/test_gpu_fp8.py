@@ -193,6 +193,25 @@ def test_zero_rows_and_extreme_scales(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 16, 40, 2100])
+def test_a_scale_of_255_is_nan(M):
+    """E8M0's NaN in a caller's own scales reaches exactly the outputs that its block enters."""
+    K, N = 384, 144
+    g = torch.Generator().manual_seed(3)
+    a = ops.fp8_quantize(torch.randn(M, K, generator=g).to(torch.bfloat16).cuda())
+    w = ops.fp8_quantize(torch.randn(N, K, generator=g).to(torch.bfloat16).cuda(), 128)
+    sa, sw = a.scales.clone(), w.scales.clone()
+    sa[M // 2, 1] = 255
+    sw[1, 2] = 255  # rows 128 .. 143 of the weight
+    out = ops.gemm_fp8(ops.Fp8Tensor(a.q, sa), ops.Fp8Tensor(w.q, sw, 128))
+    want = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    want[M // 2] = True
+    want[:, 128:] = True
+    assert torch.equal(out.isnan(), want)
+    assert ops.Fp8Tensor(a.q, sa).dequantize().isnan().sum() == 128
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [5, 700, 3000])
 def test_replays_from_a_graph_and_on_another_stream(M):
     N, K = 520, 1152
