@@ -56,7 +56,8 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
     """The 8-bit image of a projection weight (a scale for each 128 x 128 block), quantised once and kept on the module
     until the parameter is modified (other than through ``.data``, which leaves no trace), replaced or moved.  The entry
     holds the weight's storage, so that no other weight can turn up at its address, and the host waits for the one
-    quantisation, so that every stream may use it.  Not kept, but made by every call: under a stream capture (the image would
+    quantisation, so that every stream may use it; graphs captured with it follow a changed weight once a forward outside
+    of them has seen the change.  Not kept, but made by every call: under a stream capture (the image would
     exist from the first replay on) and for inference tensors (whose changes are not counted)."""
     if w2d.is_inference():
         return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
@@ -64,11 +65,15 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
     tag = (w2d.data_ptr(), w2d._version, tuple(w2d.shape))
     entry = cache.get(key)
     if entry is None or entry[0] != tag:
-        entry = (tag, ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK), w2d.detach())
+        image = ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
         if torch.cuda.is_current_stream_capturing():
-            return entry[1]
+            return image
+        if entry is not None and entry[0][2] == tag[2] and entry[1].q.device == w2d.device:
+            entry[1].q.copy_(image.q)  # in place: captured graphs read from there
+            entry[1].scales.copy_(image.scales)
+            image = entry[1]
         torch.cuda.current_stream(w2d.device).synchronize()
-        cache[key] = entry
+        entry = cache[key] = (tag, image, w2d.detach())
     return entry[1]
 
 

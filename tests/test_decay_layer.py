@@ -139,6 +139,23 @@ def test_a_capture_without_warm_up_keeps_nothing():
 
 
 @pytest.mark.gpu
+def test_a_captured_forward_follows_a_changed_weight():
+    m = layer()
+    m.fp8 = True
+    x = torch.randn(1, 70, 192).to(BF16).cuda()
+    before = m(x)[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, _ = m(x)
+    with torch.no_grad():
+        m.proj.weight.mul_(-2)
+    eager = m(x)[0]
+    junk = [torch.full_like(m.proj.weight, 3.0) for _ in range(8)]  # would land in memory that had been freed
+    g.replay()
+    assert torch.equal(y, eager) and not torch.equal(y, before) and len(junk) == 8
+
+
+@pytest.mark.gpu
 def test_block_with_8_bit_projections():
     """Every operand is off by at most 2^-4 of itself (rms 2^-4 / sqrt 3), so a projection by sqrt 2 of that in norm; four
     projections follow one another in the block, and their branches' share of the output is at most all of it."""
