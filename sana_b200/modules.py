@@ -441,7 +441,8 @@ class DecayCausalAttention(nn.Module):
     def _apply(self, fn, *args, **kwargs):
         kept = self.log_decay.data
         super()._apply(fn, *args, **kwargs)
-        self.log_decay.data = kept.to(device=self.log_decay.device, dtype=torch.float32)
+        source = self.log_decay.data if kept.is_meta else kept  # nothing to keep before the module has memory
+        self.log_decay.data = source.to(device=self.log_decay.device, dtype=torch.float32)
         return self
 
     def _split(self, x2d: torch.Tensor):

@@ -23,6 +23,12 @@ def test_layer_keeps_its_decays_in_fp32_and_refuses_what_the_kernels_lack():
     assert m.log_decay.dtype == torch.float32 and torch.equal(m.log_decay, before) and m.qkv.weight.dtype == BF16
     assert (m.log_decay < 0).all()
     assert set(m.state_dict()) == {"log_decay", "qkv.weight", "proj.weight", "proj.bias"}
+    with torch.device("meta"):
+        empty = sana_b200.DecayCausalAttention(64, 64, 2).to(BF16)
+    empty = empty.to_empty(device="cpu")
+    assert empty.log_decay.dtype == torch.float32 and empty.qkv.weight.dtype == BF16
+    empty.load_state_dict(m.state_dict())
+    assert torch.equal(empty.log_decay, before)
     for kw in (dict(heads=3), dict(heads=8), dict(heads=2, kv_heads=3)):
         with pytest.raises(NotImplementedError):
             sana_b200.DecayCausalAttention(64, 64, **kw)
