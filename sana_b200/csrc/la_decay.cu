@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(256) la_decay_f32_kernel(const LdArgs a) {
 // ---- one token -----------------------------------------------------------------------------------------------------
 // A CTA holds the state of one head of one sequence: reads it once, adds the token, writes it back and multiplies it
 // with q on the way.  Bound by the state's bytes (8 (D+1) D per head against 4 D^2 operations): 256 sequences of 16 heads of 128
-// channels (a state of 270 MB, read and written) 106 us, 5.1 TB/s.  GP lanes share a row; all rows of a thread are in flight at once.
+// channels (a state of 270 MB, read and written) 83 us, 6.5 TB/s, the copy rate.  GP lanes share a row; all rows of a thread
+// are in flight at once, q, k and v with them (loaded behind the test for repeated slots they cost 12 us).
 struct LdStepArgs {
   const void *q, *k, *v;
   int64_t ldq, ldk, ldv;
@@ -568,13 +569,16 @@ struct LdStepArgs {
   int relu, normalise;
 };
 
+// About eight float4 of the state per thread, so that an SM's CTAs have some 130 KB of it in flight: with 256 threads for
+// every width, 256 sequences of 20 heads of 112 took 96 us instead of 83, of 70 heads of 32 channels 45 instead of 25.
+constexpr int ld_step_threads(int D) { return D >= 80 ? 512 : D >= 64 ? 256 : D >= 48 ? 128 : 64; }
 template <int D, typename T>
-__global__ void __launch_bounds__(256) la_decay_step_kernel(const LdStepArgs a) {
+__global__ void __launch_bounds__(ld_step_threads(D)) la_decay_step_kernel(const LdStepArgs a) {
   constexpr int V = D / 4;                                                 // float4 pieces of a row
   constexpr int GP = V <= 4 ? 4 : V <= 8 ? 8 : V <= 16 ? 16 : 32;          // lanes per row
-  constexpr int RPI = 256 / GP;                                            // rows per pass of the CTA
+  constexpr int RPI = ld_step_threads(D) / GP;                                            // rows per pass of the CTA
   constexpr int PASSES = (D + 1 + RPI - 1) / RPI;
-  __shared__ float o_s[D + 1];
+  __shared__ float o_s[D + 1], v_s[D + 1];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int slot = a.slots ? a.slots[b] : b;
   T* out = static_cast<T*>(a.out) + (int64_t)b * a.ldo + (int64_t)h * D;
@@ -591,15 +595,7 @@ __global__ void __launch_bounds__(256) la_decay_step_kernel(const LdStepArgs a) 
     const int r = r0 + p * RPI;
     s[p] = in && r <= D ? *reinterpret_cast<const float4*>(S + (int64_t)r * D) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  // a slot that an earlier row of the batch already names would be updated by two CTAs at once: such a row is not a
-  // step of its own, its output is NaN and the state takes the first row's token only
-  bool twice = false;
-  if (a.slots)
-    for (int i = tid; i < b; i += 256) twice |= a.slots[i] == slot;
-  if (__syncthreads_or(twice)) {
-    if (tid < D) out[tid] = from_f32<T>(__uint_as_float(0x7fffffffu));
-    return;
-  }
+  // q, k and v are under way with the state
   const float lam = expf(a.log_decay[h]);
   const int hk = h / a.group;
   const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.ldq + (int64_t)h * D;
@@ -612,10 +608,20 @@ __global__ void __launch_bounds__(256) la_decay_step_kernel(const LdStepArgs a) 
     k[e] = in ? to_f32(kp[4 * l + e]) : 0.f;
     if (a.relu) q[e] = q[e] < 0.f ? 0.f : q[e], k[e] = k[e] < 0.f ? 0.f : k[e];
   }
+  if (tid <= D) v_s[tid] = tid < D ? to_f32(vp[tid]) : 1.f;
+  // a slot that an earlier row of the batch already names would be updated by two CTAs at once: such a row is not a
+  // step of its own, its output is NaN and the state takes the first row's token only
+  bool twice = false;
+  if (a.slots)
+    for (int i = tid; i < b; i += ld_step_threads(D)) twice |= a.slots[i] == slot;
+  if (__syncthreads_or(twice)) {
+    if (tid < D) out[tid] = from_f32<T>(__uint_as_float(0x7fffffffu));
+    return;
+  }
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int r = r0 + p * RPI;
-    const float v = r < D ? to_f32(vp[r]) : 1.f;
+    const float v = v_s[r <= D ? r : D];
     float4 n;
     n.x = fmaf(v, k[0], lam * s[p].x);
     n.y = fmaf(v, k[1], lam * s[p].y);
@@ -698,8 +704,8 @@ static int launch_decay(LdArgs& a, int64_t B, int dtype, int64_t workspace_bytes
 template <int D>
 static int launch_decay_step(const LdStepArgs& a, int64_t B, int dtype, cudaStream_t st) {
   const dim3 grid((unsigned)a.H, (unsigned)B);
-  if (dtype == SANA_BF16) la_decay_step_kernel<D, __nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  else la_decay_step_kernel<D, float><<<grid, 256, 0, st>>>(a);
+  if (dtype == SANA_BF16) la_decay_step_kernel<D, __nv_bfloat16><<<grid, ld_step_threads(D), 0, st>>>(a);
+  else la_decay_step_kernel<D, float><<<grid, ld_step_threads(D), 0, st>>>(a);
   SANA_LAUNCH_CHECK("la_decay_step kernel");
   return SANA_OK;
 }
