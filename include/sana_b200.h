@@ -257,8 +257,13 @@ int sana_la_rope_take_device_status(int* status_out);
  *   rows behind them hold has no effect, their outputs are zeros, and the state is the one after token lengths[b] - 1 (or prior, or zeros)
  *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
  *   arguments), 16-byte aligned.
- * State, decays and normalisers are fp32; bf16: both sides of the products are bf16, the state enters the product with q
- * as two bf16 terms and is updated with v in three, the scores are rounded to bf16 once (64 tokens or fewer: two terms).  Bit-reproducible.  An infinity or
+ * State, decays and normalisers are fp32.  Both sides of the bf16 products are bf16, and what was fp32 enters them as a sum
+ * of bf16 terms (one: off by 2^-8 of the value at most, two: 2^-17, three: 2^-24):
+ *                                     up to 64 tokens     more
+ *   state, with q                     two                 one; its key sum two
+ *   decayed scores, with v            two                 one (their sum, for the normaliser: fp32)
+ *   decayed tokens, in the update     v in three          k in three; two where the state only serves the outputs
+ * Bit-reproducible.  An infinity or
  * NaN in v gives NaN in its channel from its token on, one in k or q what the sums make of it; no output before the
  * token is touched.
  *

@@ -252,7 +252,11 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           if (held(i)) dst[row_of(i) * D + sj] = fmaf(f, S[i], n_end > n_begin ? __ldg(src + row_of(i) * D + sj) : 0.f);
       }
     }
-    // row j of the state operand, 8 value channels to a 16-byte piece
+    // Row j of the state operand, 8 value channels to a 16-byte piece.  The value channels enter as one bf16 term (2^-8 of each
+    // at most, of either sign, summed over D key channels): a second one would double these products and their operand, which
+    // shared memory has no room for next to the second v tile.  The key sum, whose error all channels of an output would share,
+    // enters as two (2^-17): the second takes a column of the padding.
+    auto key_sum = [](float z) -> uint32_t { return pack_bf16(z, z - __bfloat162float(__float2bfloat16_rn(z))); };
     auto write_operand = [&]() {
       if constexpr (T::STACK) {
         unsigned char* row = smem + T::OFF_S + lane * 128;
@@ -260,7 +264,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (lane < D && 8 * warp < D)
           put(warp, make_uint4(pack_bf16(S[0], S[1]), pack_bf16(S[2], S[3]), pack_bf16(S[4], S[5]), pack_bf16(S[6], S[7])));
         if (lane < D && warp == 3) {
-          put(D / 8, make_uint4(pack_bf16(S[8], 0.f), 0u, 0u, 0u));
+          put(D / 8, make_uint4(key_sum(S[8]), 0u, 0u, 0u));
           put(D / 8 + 1, make_uint4(0u, 0u, 0u, 0u));
         }
       } else if (jin) {
@@ -271,7 +275,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 8 * c + 2 * e;
-            w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? pack_bf16(S[NS - 1], 0.f) : 0u;
+            w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? key_sum(S[NS - 1]) : 0u;
           }
           *reinterpret_cast<uint4*>(row + (c >> 3) * T::STATE_BLK + (((c & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -348,9 +352,11 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         float m = a.scale;
         if (a.normalise) {
           if (!lt_wait(rsready + 8 * ph, (uint32_t)(c >> 1) & 1u, abort_flag, 3)) { ok = false; break; }
-          const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D));
+          const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D));      // q with the key sum: its first term,
+          const uint32_t d2 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D + 1));  // its second
           tmem_ld_wait();
-          m = 1.f / (fmaf(f, __uint_as_float(d1), reinterpret_cast<const float*>(smem + T::OFF_RS)[(c & 1) * C + t]) + a.eps);
+          m = 1.f / (fmaf(f, __uint_as_float(d1) + __uint_as_float(d2),
+                          reinterpret_cast<const float*>(smem + T::OFF_RS)[(c & 1) * C + t]) + a.eps);
         }
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row0 + n0 + t) * a.ldo + (int64_t)h * D;
         uint32_t x[16], y[16];
