@@ -62,7 +62,7 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
     if w2d.is_inference():
         return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
     cache = owner.__dict__.setdefault("_fp8_weights", {})
-    tag = (w2d.data_ptr(), w2d._version, tuple(w2d.shape))
+    tag = (w2d.data_ptr(), w2d._version, w2d.shape, w2d.stride(), w2d.dtype)
     entry = cache.get(key)
     if entry is None or entry[0] != tag:
         image = ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
