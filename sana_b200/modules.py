@@ -56,9 +56,11 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
     """The 8-bit image of a projection weight (a scale for each 128 x 128 block), quantised once and kept on the module
     until the parameter is modified (other than through ``.data``, which leaves no trace), replaced or moved.  The entry
     holds the weight's storage, so that no other weight can turn up at its address, and the host waits for the one
-    quantisation, so that every stream may use it; graphs captured with it follow a changed weight once a forward outside
-    of them has seen the change.  Not kept, but made by every call: under a stream capture (the image would
-    exist from the first replay on) and for inference tensors (whose changes are not counted)."""
+    quantisation, so that every stream may use it.  An old image is overwritten or given up once the device has finished all
+    work that may read it.  A changed weight of the same shape is quantised into the old one's buffers; graphs captured
+    with it follow the change once a forward outside of them has seen it (no replay may run at the same time as that
+    forward).  Not kept, but made by every call: under a stream capture (the image would exist from the first replay on)
+    and for inference tensors (whose changes are not counted)."""
     if w2d.is_inference():
         return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
     cache = owner.__dict__.setdefault("_fp8_weights", {})
@@ -68,10 +70,12 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
         image = ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
         if torch.cuda.is_current_stream_capturing():
             return image
-        if entry is not None and entry[0][2] == tag[2] and entry[1].q.device == w2d.device:
-            entry[1].q.copy_(image.q)  # in place: captured graphs read from there
-            entry[1].scales.copy_(image.scales)
-            image = entry[1]
+        if entry is not None:
+            torch.cuda.synchronize(entry[1].q.device)  # products on other streams, and replays, may be reading the old image
+            if entry[0][2] == tag[2] and entry[1].q.device == w2d.device:
+                entry[1].q.copy_(image.q)  # in place: captured graphs read from there
+                entry[1].scales.copy_(image.scales)
+                image = entry[1]
         torch.cuda.current_stream(w2d.device).synchronize()
         entry = cache[key] = (tag, image, w2d.detach())
     return entry[1]

@@ -32,3 +32,26 @@ def test_a_view_of_the_weight_is_another_weight():
     fresh.proj.weight = torch.nn.Parameter(m.proj.weight.detach().contiguous().clone(), requires_grad=False)
     after = m(x)[0]
     assert torch.equal(after, fresh(x)[0]) and not torch.equal(after, before)
+
+
+@pytest.mark.gpu
+def test_a_replaced_weight_does_not_reach_a_forward_that_is_under_way():
+    """A forward queued on another stream multiplies with the weight it was called with."""
+    m, x, side = layer(), inputs(), torch.cuda.Stream()
+    weights = [m.proj.weight] + [torch.nn.Parameter(f * m.proj.weight.detach(), requires_grad=False) for f in (-2, 3)]
+    want, got = [], []
+    for w in weights:
+        m.proj.weight = w
+        want.append(m(x)[0])
+    for _ in range(2):  # the first time round everything is loaded and allocated, which may wait for the GPU
+        for w in weights:
+            m.proj.weight = w
+            m(x)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(100_000_000)  # about 50 ms
+                got.append(m(x)[0])
+    m.proj.weight = weights[0]
+    m(x)  # while the last one is still under way
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want + want))
