@@ -59,16 +59,18 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
     quantisation, so that every stream may use it.  An old image is overwritten or given up once the device has finished all
     work that may read it.  A changed weight of the same shape is quantised into the old one's buffers; graphs captured
     with it follow the change once a forward outside of them has seen it (no replay may run at the same time as that
-    forward).  Not kept, but made by every call: under a stream capture (the image would exist from the first replay on)
-    and for inference tensors (whose changes are not counted)."""
+    forward).  An image that a capture has read stays for its graph when a weight of another shape, or on another device,
+    takes its place.  Not kept, but made by every call: under a stream capture (the image would exist from the first
+    replay on) and for inference tensors (whose changes are not counted)."""
     if w2d.is_inference():
         return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
     cache = owner.__dict__.setdefault("_fp8_weights", {})
     tag = (w2d.data_ptr(), w2d._version, w2d.shape, w2d.stride(), w2d.dtype)
     entry = cache.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
     if entry is None or entry[0] != tag:
         image = ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
             return image
         if entry is not None:
             torch.cuda.synchronize(entry[1].q.device)  # products on other streams, and replays, may be reading the old image
@@ -78,6 +80,10 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
                 image = entry[1]
         torch.cuda.current_stream(w2d.device).synchronize()
         entry = cache[key] = (tag, image, w2d.detach())
+    elif capturing:  # no weight has been changed since: the graph reads the kept image
+        read = owner.__dict__.setdefault("_fp8_captured", [])
+        if not any(image is entry[1] for image in read):
+            read.append(entry[1])
     return entry[1]
 
 

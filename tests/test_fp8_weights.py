@@ -55,3 +55,19 @@ def test_a_replaced_weight_does_not_reach_a_forward_that_is_under_way():
     m(x)  # while the last one is still under way
     torch.cuda.synchronize()
     assert all(torch.equal(g, w) for g, w in zip(got, want + want))
+
+
+@pytest.mark.gpu
+def test_a_captured_forward_keeps_the_image_it_reads():
+    m, x = layer(), inputs()
+    before = m(x)[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, _ = m(x)
+    old = m.proj  # the graph reads its bias
+    m.proj = torch.nn.Linear(256, 512).to("cuda", BF16)
+    assert m(x)[0].shape[-1] == 512
+    image = 256 * 256
+    junk = [torch.full((image,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(64)]  # would land in freed memory
+    g.replay()
+    assert torch.equal(y, before) and len(junk) == 64 and old is not None
