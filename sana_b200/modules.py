@@ -19,6 +19,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import ops
 from .sharding import SequenceShard
@@ -52,23 +53,52 @@ def _fp4_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.NvFp4Tens
     return entry[1]
 
 
+class _Fp8Images(dict):
+    """The kept images of a module: key -> (tag, image, weak reference to the weight's storage), and those that captures
+    have read.  A copy of the module, or a saved one, starts without."""
+
+    def __init__(self):
+        super().__init__()
+        self.captured = []
+
+    def __deepcopy__(self, memo):
+        return _Fp8Images()
+
+    def __reduce__(self):
+        return _Fp8Images, ()
+
+
+class _ProjectionOwner(nn.Module):
+    """Base of the modules whose projections go through :func:`_project`."""
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        images = self.__dict__.get("_fp8_weights", {})
+        for key in [k for k, (_, _, weight) in images.items() if weight.expired()]:  # moved: its image goes too
+            torch.cuda.synchronize(images[key][1].q.device)  # once nothing reads it any more
+            del images[key]
+        return self
+
+
 def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor":
     """The 8-bit image of a projection weight (a scale for each 128 x 128 block), quantised once and kept on the module
     until the parameter is modified (other than through ``.data``, which leaves no trace), replaced or moved.  The entry
-    holds the weight's storage, so that no other weight can turn up at its address, and the host waits for the one
-    quantisation, so that every stream may use it.  An old image is overwritten or given up once the device has finished all
-    work that may read it.  A changed weight of the same shape is quantised into the old one's buffers; graphs captured
-    with it follow the change once a forward outside of them has seen it (no replay may run at the same time as that
-    forward).  An image that a capture has read stays for its graph when a weight of another shape, or on another device,
-    takes its place.  Not kept, but made by every call: under a stream capture (the image would exist from the first
-    replay on) and for inference tensors (whose changes are not counted)."""
+    knows whether the weight's storage still exists, so that no other weight can pass for it at its address, and the host
+    waits for the one quantisation, so that every stream may use it.  An old image is overwritten or given up once the
+    device has finished all work that may read it.  A changed weight of the same shape is quantised into the old one's
+    buffers; graphs captured with it follow the change once a forward outside of them has seen it (no replay may run at
+    the same time as that forward).  An image that a capture has read stays for its graph when a weight of another shape,
+    or on another device, takes its place.  Not kept, but made by every call: under a stream capture (the image would
+    exist from the first replay on) and for inference tensors (whose changes are not counted)."""
     if w2d.is_inference():
         return ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
-    cache = owner.__dict__.setdefault("_fp8_weights", {})
+    cache = owner.__dict__.get("_fp8_weights")
+    if cache is None:
+        cache = owner.__dict__["_fp8_weights"] = _Fp8Images()
     tag = (w2d.data_ptr(), w2d._version, w2d.shape, w2d.stride(), w2d.dtype)
     entry = cache.get(key)
     capturing = torch.cuda.is_current_stream_capturing()
-    if entry is None or entry[0] != tag:
+    if entry is None or entry[0] != tag or entry[2].expired():
         image = ops.fp8_quantize(w2d.contiguous(), ops.FP8_BLOCK)
         if capturing:
             return image
@@ -79,11 +109,9 @@ def _fp8_weight(owner: nn.Module, key: str, w2d: torch.Tensor) -> "ops.Fp8Tensor
                 entry[1].scales.copy_(image.scales)
                 image = entry[1]
         torch.cuda.current_stream(w2d.device).synchronize()
-        entry = cache[key] = (tag, image, w2d.detach())
-    elif capturing:  # no weight has been changed since: the graph reads the kept image
-        read = owner.__dict__.setdefault("_fp8_captured", [])
-        if not any(image is entry[1] for image in read):
-            read.append(entry[1])
+        entry = cache[key] = (tag, image, StorageWeakRef(w2d.untyped_storage()))
+    elif capturing and not any(image is entry[1] for image in cache.captured):
+        cache.captured.append(entry[1])
     return entry[1]
 
 
@@ -130,7 +158,7 @@ class RMSNorm(nn.Module):
         return ops.rmsnorm_(y, self.weight, float(self.eps)).reshape(x.shape)
 
 
-class LiteLA(nn.Module):
+class LiteLA(_ProjectionOwner):
     """ReLU linear attention.  Same arguments and attributes as upstream's LiteLA (which
     derives from timm's Attention: ``qkv``, ``proj``, ``num_heads``, ``scale``,
     ``attn_drop``, ``proj_drop``)."""
@@ -243,7 +271,7 @@ def wan_rotary_freqs(head_dim: int, fhw: Sequence[int], theta: float = 10000.0, 
     return torch.cat(groups, dim=-1).reshape(1, 1, f * h * w, -1)
 
 
-class LiteLAReLURope(nn.Module):
+class LiteLAReLURope(_ProjectionOwner):
     """Linear attention with the ReLU feature map first and the rotation after it, on the
     numerator's q and k only (upstream's LiteLAReLURope, sana_blocks.py:304-388; self-attention of
     Sana-Video).  Same constructor arguments, attributes and state-dict keys as upstream.
@@ -422,7 +450,7 @@ class CachedCausalAttention(LiteLAReLURope):
         return (out, kv_cache) if kv_cache is not None else out
 
 
-class DecayCausalAttention(nn.Module):
+class DecayCausalAttention(_ProjectionOwner):
     """Token-causal linear attention that forgets: ``S_t = exp(log_decay_h) S_{t-1} + [v_t; 1] phi(k_t)^T`` for each head,
     outputs ``S_t[:D] phi(q_t) / (S_t[D] . phi(q_t) + eps)`` with ReLU features (``normalize=True``, the form of
     :class:`LiteLA`) or ``D**-0.5 S_t[:D] q_t`` without.  With ``log_decay = 0`` the last token's state is LiteLA's.  No
@@ -508,7 +536,7 @@ class ConvLayer(nn.Module):
         raise NotImplementedError("ConvLayer is a parameter holder here; call GLUMBConv.forward")
 
 
-class GLUMBConv(nn.Module):
+class GLUMBConv(_ProjectionOwner):
     """Mix-FFN: 1x1 expand + SiLU, 3x3 depthwise, SiLU-GLU, 1x1 project."""
 
     def __init__(self, in_features: int, hidden_features: int, out_feature=None, kernel_size=3, stride=1,

@@ -71,3 +71,49 @@ def test_a_captured_forward_keeps_the_image_it_reads():
     junk = [torch.full((image,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(64)]  # would land in freed memory
     g.replay()
     assert torch.equal(y, before) and len(junk) == 64 and old is not None
+
+
+@pytest.mark.gpu
+def test_a_moved_module_leaves_no_memory_behind():
+    ops.gemm_fp8(ops.fp8_quantize(inputs()[0]), ops.fp8_quantize(torch.zeros(8, 192, dtype=BF16, device="cuda"), 128))
+    gc.collect()
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    m, x = layer(), inputs()
+    first = m(x)[0].cpu()
+    del x
+    m.to("cpu")
+    gc.collect()
+    assert torch.cuda.memory_allocated() == start
+    m.to("cuda")
+    assert torch.equal(m(inputs())[0].cpu(), first)
+
+
+@pytest.mark.gpu
+def test_copies_of_a_module_have_images_of_their_own():
+    m, x = layer(), inputs()
+    want = m(x)[0]
+    twin = copy.deepcopy(m)
+    with torch.no_grad():
+        twin.proj.weight.mul_(-2)
+    moved = twin(x)[0]
+    assert torch.equal(m(x)[0], want) and not torch.equal(moved, want)
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    loaded = torch.load(f, weights_only=False)
+    del m
+    gc.collect()
+    assert torch.equal(loaded(x)[0], want) and torch.equal(twin(x)[0], moved)
+
+
+def pack_of(model):
+    """A weight pack of the right names and shapes (its codes are zeros)."""
+    pack = {}
+    for name, module in model.named_modules():
+        for key, w in weight_pack._projections(module):
+            base = f"{name}.{key}.nvfp4"
+            n, k = w.shape
+            pack.update({base + ".q": torch.zeros(n, k // 2, dtype=torch.uint8), base + ".sf": torch.zeros(16, dtype=torch.uint8),
+                         base + ".scales": torch.zeros(4), base + ".shape": torch.tensor([n, k])})
+    return pack
