@@ -63,7 +63,7 @@ def pack_nvfp4_weights(model: nn.Module) -> Dict[str, torch.Tensor]:
 def load_nvfp4_weights(model: nn.Module, pack: Dict[str, torch.Tensor], enable: bool = True) -> int:
     """Installs the packed weights on the matching modules of ``model`` (moved to each module's
     device) so that their NVFP4 projections use them instead of quantising the bf16 weights, and
-    (``enable``) switches those modules to NVFP4.  Every NVFP4-capable projection of the model must
+    (``enable``) switches those modules to NVFP4 (which replaces the 8-bit setting).  Every NVFP4-capable projection of the model must
     be in the pack with the right shape.  Returns the number of projections installed."""
     n = 0
     for name, module in model.named_modules():
@@ -80,5 +80,5 @@ def load_nvfp4_weights(model: nn.Module, pack: Dict[str, torch.Tensor], enable: 
             module.__dict__.setdefault("_nvfp4_packed", {})[key] = t
             n += 1
         if enable and isinstance(module, (LiteLA, GLUMBConv)):
-            module.nvfp4 = True
+            module.nvfp4, module.fp8 = True, False
     return n

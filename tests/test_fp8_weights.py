@@ -117,3 +117,14 @@ def pack_of(model):
             pack.update({base + ".q": torch.zeros(n, k // 2, dtype=torch.uint8), base + ".sf": torch.zeros(16, dtype=torch.uint8),
                          base + ".scales": torch.zeros(4), base + ".shape": torch.tensor([n, k])})
     return pack
+
+
+def test_installed_nvfp4_weights_replace_the_8_bit_setting():
+    blk = sana_b200.SanaMSBlock(64, 2, mlp_ratio=2.5, attn_type="linear", ffn_type="glumbconv")
+    blk.set_fp8(True)
+    assert sana_b200.load_nvfp4_weights(blk, pack_of(blk), enable=False) == 4
+    assert blk.attn.fp8 and blk.mlp.fp8 and not blk.attn.nvfp4  # installed, not switched on
+    sana_b200.load_nvfp4_weights(blk, pack_of(blk))
+    assert blk.attn.nvfp4 and blk.mlp.nvfp4 and not blk.attn.fp8 and not blk.mlp.fp8
+    blk.set_fp8(True)
+    assert blk.attn.fp8 and blk.mlp.fp8 and not blk.attn.nvfp4 and not blk.mlp.nvfp4
