@@ -80,6 +80,11 @@ struct Lt {
   static constexpr int COL_DS = OUT ? COL_O1 + NV : 0;
   static constexpr int COLS = COL_DS + NV;
   static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  // arrivals that complete a phase of barrier i (their order: at the top of the kernel); kempty, without scores: k is free
+  // once the LW warps have weighted it
+  __host__ __device__ static constexpr int arrivals(int i) {
+    return !OUT && i == 5 ? LW : i < 17 ? 1 : i < 19 ? LW / 2 : i < 22 ? LW : 4;
+  }
   static constexpr int CTAS = TMEM_COLS <= 256 && 2 * (BYTES + 1024) <= 228 * 1024 && D <= 32 ? 2 : 1;  // resident per SM
   // D = f32 (bit 4), A = B = bf16 (7, 10), transposes (MN-major) at 15 / 16, N >> 3 at 17, M >> 4 at 24
   static constexpr uint32_t BASE = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
@@ -184,8 +189,7 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const int64_t per = (int64_t)(D + 1) * D;
 
   if (tid == 0) {
-    for (int i = 0; i < 29; ++i) mbar_init(bar + 8 * i, i < 17 ? 1 : i < 19 ? LW / 2 : i < 22 ? LW : 4);
-    if (!OUT) mbar_init(kempty, LW);  // no scores: k is free once it has been weighted
+    for (int i = 0; i < 29; ++i) mbar_init(bar + 8 * i, T::arrivals(i));
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
