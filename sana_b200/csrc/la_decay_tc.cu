@@ -52,7 +52,7 @@ struct Lt {
   static constexpr int WTILE = STACK ? 2 * LT_BLK : NT * KTILE;
   static constexpr int STATE_BLK = D * 128;              // bf16 state operand: rows = key channels
   static constexpr int X_BYTES = STACK ? (D + 1) * 32 * (NT == 3 ? 10 : 8) : 0;  // sums of the terms, [D+1][32]; the third in bf16
-  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 2 + 32) + (OUT ? 4 * 2 * LT_C : 0) + 240 +
+  static constexpr int SCRATCH = (OUT ? VB * STATE_BLK : 0) + X_BYTES + 4 * (32 + LT_C + 2 + 32) + (OUT ? 4 * 2 * LT_C : 0) + 248 +
                                  4 * (4 + 4 * D);
   static constexpr int ONE_EACH = WTILE + VTILE + KTILE + (OUT ? KTILE : 0) + SCRATCH;
   static constexpr int LIMIT = OUT && D <= 32 ? 113 * 1024 : 232448;  // two CTAs per SM, or one
@@ -70,7 +70,11 @@ struct Lt {
   static constexpr int OFF_BAR = OFF_RS + (OUT ? 4 * 2 * LT_C : 0);
   // Tokens whose v is not finite, by channel, for the last chunks: a flag each, then the first such token (128: none).
   static constexpr int BADS = VBUF == 2 ? 4 : 2;  // a chunk's entries are cleared before the one BADS later can be filled
-  static constexpr int OFF_BAD = OFF_BAR + 240;
+  // Barriers, then the tensor-memory address and the abort flag.  With one v tile its second barriers are free, and one of
+  // them does for bready (128 channels leave no room for another).
+  static constexpr int BARS = VBUF == 2 ? 30 : 29;
+  static constexpr int OFF_SLOT = OFF_BAR + 8 * BARS;
+  static constexpr int OFF_BAD = OFF_SLOT + 8;
   static constexpr int BYTES = OFF_BAD + 4 * (BADS + BADS * D);
   // Scores in two halves of 64 keys.  O2 has columns of its own, except for 128 channels, where it starts inside the
   // second half and the next chunk's scores wait until it has been read.
@@ -83,7 +87,7 @@ struct Lt {
   // arrivals that complete a phase of barrier i (their order: at the top of the kernel); kempty, without scores: k is free
   // once the LW warps have weighted it
   __host__ __device__ static constexpr int arrivals(int i) {
-    return !OUT && i == 5 ? LW : i < 17 ? 1 : i < 19 ? LW / 2 : i < 22 ? LW : 4;
+    return !OUT && i == 5 ? LW : VBUF == 1 && i == 7 ? 4 : i < 17 ? 1 : i < 19 ? LW / 2 : i < 22 ? LW : 4;
   }
   static constexpr int CTAS = TMEM_COLS <= 256 && 2 * (BYTES + 1024) <= 228 * 1024 && D <= 32 ? 2 : 1;  // resident per SM
   // D = f32 (bit 4), A = B = bf16 (7, 10), transposes (MN-major) at 15 / 16, N >> 3 at 17, M >> 4 at 24
@@ -153,6 +157,14 @@ __device__ __forceinline__ bool lt_wait(uint32_t bar, uint32_t parity, volatile 
   return true;
 }
 
+// whether all of the four state warps say so: a barrier of 128 threads
+__device__ __forceinline__ bool lt_all(bool mine) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((uint32_t)mine) : "memory");
+  return r != 0;
+}
+
 template <int D, int NT, bool OUT>
 __global__ void __launch_bounds__(Lt<D, NT, OUT>::THREADS, Lt<D, NT, OUT>::CTAS) 
 la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -176,8 +188,10 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const uint32_t sopread = bar + 120, oready = bar + 128;                                        // 17 of one arrival
   const uint32_t wfull = bar + 136 /* 2 */, vfull = bar + 152, qfull = bar + 160, kfull = bar + 168;
   const uint32_t pready = bar + 176 /* 2 */, rsready = bar + 192 /* 2 */, dsread = bar + 208, sopready = bar + 216, oread = bar + 224;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_BAR + 232);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_BAR + 236);
+  const uint32_t bready = T::VBUF == 2 ? bar + 232 : vempty + 8;  // the state warps have looked at a chunk's non-finite v
+  const uint32_t slot = sm + T::OFF_SLOT;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + T::OFF_SLOT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + T::OFF_SLOT + 4);
 
   const int h = blockIdx.x, seg = blockIdx.y, b = blockIdx.z;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
@@ -189,12 +203,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const int64_t per = (int64_t)(D + 1) * D;
 
   if (tid == 0) {
-    for (int i = 0; i < 29; ++i) mbar_init(bar + 8 * i, T::arrivals(i));
+    for (int i = 0; i < T::BARS; ++i) mbar_init(bar + 8 * i, T::arrivals(i));
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 232), "r"((uint32_t)T::TMEM_COLS)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"((uint32_t)T::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -290,15 +304,16 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     };
     if (OUT && chunks > 0) write_operand();
     bool ok = true;
+    uint32_t bphase = 0u;
     for (int c = 0; c < chunks; ++c) {
       const uint32_t ph = (uint32_t)(c & 1);
       const int n0 = n_begin + c * C, nv = min(C, n_end - n0);
-      if (!lt_wait(dsready, ph, abort_flag, 1)) { ok = false; break; }
+      ok = ok && lt_wait(dsready, ph, abort_flag, 1);
       tcgen05_fence_after();
       if constexpr (T::STACK) {  // warp s holds the sum of term s, lane = key channel: through shared memory, then warp by channels
         float* x = reinterpret_cast<float*>(smem + T::OFF_X) + lane;
         __nv_bfloat16* x3 = reinterpret_cast<__nv_bfloat16*>(smem + T::OFF_X + 2 * (D + 1) * 32 * 4) + lane;
-        if (warp < NT) {
+        if (ok && warp < NT) {
           uint32_t d[NV];
 #pragma unroll
           for (int g = 0; g < D / 16; ++g) tmem_ld_32x16(tmem + lanes + (uint32_t)(T::COL_DS + 16 * g), *reinterpret_cast<uint32_t(*)[16]>(d + 16 * g));
@@ -310,7 +325,10 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             else x3[i * 32] = __float2bfloat16_rn(__uint_as_float(d[i]));  // 2^-16 of the first: its rounding is below 2^-24
           }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the scratch is free again once every warp has arrived at dsread
+        // The four warps go on or leave together.  A named barrier (an mbarrier cost 3 % more), which always fills:
+        // whatever a warp's waits say, each of them ends, and nothing but this leaves the loop before its last chunk.
+        ok = lt_all(ok);  // the scratch is free again once every warp has arrived at dsread
+        if (!ok) break;
         const float whole = pow_s[nv];
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -319,6 +337,8 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (NT == 3) r += __bfloat162float(x3[row_of(i) * 32]);
             S[i] = fmaf(whole, S[i], x[row_of(i) * 32] + r);
           }
+      } else if (!ok) {
+        break;
       } else if (warp_in) {
         const float whole = pow_s[nv];
         uint32_t d[2][16];  // the next columns are under way while these are added
@@ -347,15 +367,15 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (lane == 0) mbar_arrive(dsread);
       if (OUT) {
         if (c + 1 < chunks) {
-          if (!lt_wait(sopread, ph, abort_flag, 2)) { ok = false; break; }
+          if (!lt_wait(sopread, ph, abort_flag, 2)) { ok = false; continue; }
           write_operand();
         }
-        if (!lt_wait(oready, ph, abort_flag, 3)) { ok = false; break; }
+        if (!lt_wait(oready, ph, abort_flag, 3)) { ok = false; continue; }
         tcgen05_fence_after();
         const float f = pow_s[t + 1];
         float m = a.scale;
         if (a.normalise) {
-          if (!lt_wait(rsready + 8 * ph, (uint32_t)(c >> 1) & 1u, abort_flag, 3)) { ok = false; break; }
+          if (!lt_wait(rsready + 8 * ph, (uint32_t)(c >> 1) & 1u, abort_flag, 3)) { ok = false; continue; }
           const uint32_t d1 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D));      // q with the key sum: its first term,
           const uint32_t d2 = lt_ld1(tmem + lanes + (uint32_t)(T::COL_O1 + D + 1));  // its second
           tmem_ld_wait();
@@ -403,7 +423,10 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           lt_arrived(y);
         }
         if (poisoned) {
-          asm volatile("bar.sync 2, 128;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bready);
+          if (!lt_wait(bready, bphase, abort_flag, 21)) { ok = false; continue; }
+          bphase ^= 1u;
           for (int i = tid; i < D; i += 128) bad_from[c % T::BADS * D + i] = C;
           if (tid == 0) *bad = 0;
           __threadfence_block();
