@@ -291,10 +291,6 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) {  // give copies in flight time to land before shared memory is released
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) {}
-      }
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer ---------------------------------------
@@ -402,6 +398,10 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   }
 
   __syncwarp();
+  if (*abort_flag) {  // give copies and products in flight time to end before shared and tensor memory are released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {}
+  }
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -516,10 +516,6 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           tma_load_2d_pair(sa + P8_A_BYTES, &tmB, fb, kb * F8_BK, n0);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
-      }
-      if (!ok) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) {}
       }
     }
   } else if (warp == 1) {
@@ -642,6 +638,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   }
 
   __syncwarp();
+  if (*abort_flag) {  // give copies and products in flight time to end before shared and tensor memory are released
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {}
+  }
   tcgen05_fence_before();
   __syncthreads();
   cluster_sync_all();  // nobody leaves while the other CTA may still signal or read it

@@ -31,3 +31,16 @@ def test_no_role_waits_without_a_limit():
     # behind it: out of the loop at once when it says so (heads that do not meet there leave alone), else only to the next chunk
     assert re.match(r";\s*if \(!ok\) break;", after) and len(re.findall(r"\bbreak\b", after)) == 2 and "return" not in after
     assert re.search(r"else if \(!ok\) \{\s*break;", after)
+
+
+def test_a_kernel_that_gives_up_lets_its_copies_and_products_end():
+    """Whichever role's wait ran out: before the last rendezvous all warps look at the flag and leave time for the copies
+    into shared memory and the products into tensor memory that are still under way."""
+    pause = re.compile(r"if \(\*abort_flag\) \{\s*const long long t0 = clock64\(\);\s*while \(clock64\(\) - t0 < 2000000LL\) \{\}\s*\}")
+    for name, kernels in (("la_decay_tc.cu", 1), ("gemm_fp8.cu", 2)):
+        src = code(name)
+        ends = [m.start() for m in re.finditer(r"tcgen05\.dealloc", src)]
+        assert len(ends) == kernels
+        for e in ends:
+            last_sync = src.rindex("__syncthreads()", 0, e)
+            assert any(0 < last_sync - m.end() < 200 for m in pause.finditer(src)), (name, e)
