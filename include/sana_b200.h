@@ -250,7 +250,8 @@ int sana_la_rope_take_device_status(int* status_out);
  * is theirs, in the layout of sana_la_rope_state.  No counterpart upstream (its causal attention, sana_blocks.py:391-572,
  * is causal over whole chunks of frames and keeps everything).
  *   q, out [B*N, *] rows of H*D channels (head-major), k, v [B*N, *] rows of Hk*D channels; H a
- *   multiple of Hk (query head h reads key/value head h / (H / Hk)); D a multiple of 16 in [16, 128]; rows 16-byte aligned
+ *   multiple of Hk (query head h reads key/value head h / (H / Hk)); D a multiple of 16 in [16, 128]; rows 16-byte aligned; out may be q
+ *   itself (pointer and stride) and must not overlap q, k or v otherwise (not checked here)
  *   log_decay [H] fp32;  prior [B, H, D+1, D] fp32 (the state before the first token) or NULL;  state: the state after
  *   the last token, a buffer other than prior
  *   lengths [B] int32 on the device, or NULL: sequence b has lengths[b] tokens (clamped to [0, N]); what the

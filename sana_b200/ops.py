@@ -872,6 +872,29 @@ def _int32_vector(t: Optional[torch.Tensor], n: int, what: str) -> Optional[int]
     return t.data_ptr()
 
 
+def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two row views (contiguous rows of one element size) may share an element.  Views of one row stride are
+    compared by their columns, as neighbouring column blocks of one buffer lie in each other's spans; with different strides
+    overlapping spans count."""
+    es = a.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    sa, sb = a.stride(0) * es, b.stride(0) * es
+    wa, wb = a.shape[1] * es, b.shape[1] * es
+    if pa + (a.shape[0] - 1) * sa + wa <= pb or pb + (b.shape[0] - 1) * sb + wb <= pa:
+        return False
+    if sa != sb or sa <= 0 or a.shape[0] == 1 or b.shape[0] == 1:
+        return True
+    d = (pb - pa) % sa
+    return d < wa or sa - d < wb
+
+
+def _check_out_place(what: str, out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Other rows and heads read k and v, and their own part of q, while an output is written."""
+    same = out.data_ptr() == q.data_ptr() and (out.stride(0) == q.stride(0) or out.shape[0] == 1)
+    if _rows_overlap(out, k) or _rows_overlap(out, v) or not same and _rows_overlap(out, q):
+        raise SanaLibraryError(f"{what}: out may take the place of q, but not overlap it otherwise, nor k or v")
+
+
 def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, B: int, N: int, H: int, D: int,
              scale: float = 1.0, relu: bool = False, eps: Optional[float] = None, prior: Optional[torch.Tensor] = None,
              lengths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -881,7 +904,7 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
 
     q [B*N, H*D] and k, v [B*N, Hk*D] views (column blocks of a projection), H a multiple of Hk; log_decay fp32 [H], not
     positive; prior fp32 [B, H, D+1, D], the state carried in; lengths int32 [B] for a padded batch (rows behind a
-    sequence give zeros); out must not overlap k or v.  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
+    sequence give zeros); out may be q itself, and must not overlap q, k or v otherwise.  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
     dev = _device_of("la_decay", q, k, v, log_decay, prior, lengths, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -893,11 +916,14 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
     if prior is not None and (prior.shape != (B, H, D + 1, D) or prior.dtype != torch.float32 or not prior.is_contiguous()):
         raise SanaLibraryError("la_decay: prior must be contiguous fp32 [B, H, D+1, D]")
     lens = _int32_vector(lengths, B, "la_decay: lengths")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(B * N, H * D, dtype=q.dtype, device=q.device)
     ro, co, ldo = _rows2d(out, "la_decay out")
     if ro != B * N or co != H * D or out.dtype != q.dtype:
         raise SanaLibraryError("la_decay: bad output tensor")
+    if given:
+        _check_out_place("la_decay", out, q, k, v)
     lib = _lib.load()
     state = torch.empty(B, H, D + 1, D, dtype=torch.float32, device=q.device)
     ws_bytes = lib.sana_la_decay_workspace_bytes(B, N, H, D, dt)
@@ -919,7 +945,7 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
     """One token of each of B sequences through :func:`la_decay`'s recurrence: q [B, H*D], k, v [B, Hk*D]; ``state`` fp32
     [pool, H, D+1, D] is updated in place, row b using entry ``slots[b]`` (int32 [B]; without it, entry b).  A slot of -1
     marks an unused row (output zeros); a slot outside the pool, or one an earlier row names already, gives NaN outputs
-    and leaves the state alone; out must not overlap k or v.  Returns out [B, H*D]."""
+    and leaves the state alone; out as for :func:`la_decay`.  Returns out [B, H*D]."""
     dev = _device_of("la_decay_step", q, k, v, log_decay, state, slots, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -933,11 +959,14 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
     if slots is None and state.shape[0] != B:
         raise SanaLibraryError("la_decay_step: without slots the state must hold one entry per row")
     ids = _int32_vector(slots, B, "la_decay_step: slots")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(B, H * D, dtype=q.dtype, device=q.device)
     ro, co, ldo = _rows2d(out, "la_decay_step out")
     if ro != B or co != H * D or out.dtype != q.dtype:
         raise SanaLibraryError("la_decay_step: bad output tensor")
+    if given:
+        _check_out_place("la_decay_step", out, q, k, v)
     _lib.check(_lib.load().sana_la_decay_step(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
                                               state.data_ptr(), state.shape[0], ids, out.data_ptr(), ldo if B > 1 else max(ldo, co),
                                               B, H, Hk, D, scale, 1 if relu else 0, -1.0 if eps is None else eps,
