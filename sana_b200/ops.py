@@ -504,7 +504,7 @@ def _epilogue(M: int, Nn: int, dtype, bias, act, relu_cols, gate, residual):
         Mr, Nr, ldr = _rows2d(residual, "gemm residual")
         if Mr != M or Nr != Nn or residual.dtype != dtype:
             raise SanaLibraryError("gemm: residual must be [M, N] in the output dtype")
-        ep.residual, ep.ldr = residual.data_ptr(), ldr
+        ep.residual, ep.ldr = residual.data_ptr(), ldr if M > 1 else Nn
     return ep, keep
 
 
@@ -805,7 +805,7 @@ def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8Tensor:
     q = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=x.device)
     words = (kb + 3) // 4 * 4
     sf = torch.empty((rows + block_rows - 1) // block_rows, words, dtype=torch.uint8, device=x.device)
-    _lib.check(_lib.load().sana_fp8_quantize(x.data_ptr(), ld if rows > 1 else max(ld, K), q.data_ptr(), sf.data_ptr(), words,
+    _lib.check(_lib.load().sana_fp8_quantize(x.data_ptr(), ld if rows > 1 else K, q.data_ptr(), sf.data_ptr(), words,
                                              rows, K, block_rows, _dtype_code(x.dtype), _stream_of(dev)), "sana_fp8_quantize")
     counters.launches += 1
     return Fp8Tensor._of(q, sf[:, :kb], block_rows, rows, K)
@@ -827,6 +827,8 @@ def gemm_fp8(a: Fp8Tensor, w: Fp8Tensor, bias=None, act: int = ACT_NONE, relu_co
     Mo, No, ldo = _rows2d(out, "gemm_fp8 out")
     if Mo != M or No != Nn or out.dtype != torch.bfloat16:
         raise SanaLibraryError("gemm_fp8: bad output tensor")
+    if M == 1:  # as with a single row of q: its stride is never used
+        ldo = Nn
     ep = keep = None
     if bias is not None or act != ACT_NONE or gate is not None or residual is not None:
         ep, keep = _epilogue(M, Nn, torch.bfloat16, bias, act, relu_cols, gate, residual)
@@ -932,7 +934,7 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _lib.check(lib.sana_la_decay(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
                                  prior.data_ptr() if prior is not None else None, lens, state.data_ptr(), out.data_ptr(),
-                                 ldo if ro > 1 else max(ldo, co),
+                                 ldo if ro > 1 else co,
                                  ws.data_ptr() if ws is not None else None, ws_bytes, B, N, H, Hk, D, scale, 1 if relu else 0,
                                  -1.0 if eps is None else eps, dt, _stream_of(dev)), "sana_la_decay")
     counters.launches += 2 if ws_bytes else 1
@@ -968,7 +970,7 @@ def la_decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: 
     if given:
         _check_out_place("la_decay_step", out, q, k, v)
     _lib.check(_lib.load().sana_la_decay_step(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, log_decay.data_ptr(),
-                                              state.data_ptr(), state.shape[0], ids, out.data_ptr(), ldo if B > 1 else max(ldo, co),
+                                              state.data_ptr(), state.shape[0], ids, out.data_ptr(), ldo if B > 1 else co,
                                               B, H, Hk, D, scale, 1 if relu else 0, -1.0 if eps is None else eps,
                                               _dtype_code(q.dtype), _stream_of(dev)), "sana_la_decay_step")
     counters.launches += 1

@@ -67,3 +67,21 @@ def test_outputs_over_other_inputs_are_refused(dtype):
     with pytest.raises(SanaLibraryError):
         ops.la_decay(q, k, v, ld, B, N, H, D, out=one)
     assert torch.equal(hold, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_stride_of_a_single_row_is_not_looked_at(dtype):
+    H, D = 2, 32
+    odd = lambda n: torch.randn(1, n + 13, device="cuda").to(dtype)[:, :n]  # stride n + 13
+    q, k, v, ld = odd(H * D), odd(H * D), odd(H * D), -torch.rand(H).cuda()
+    want, st = ops.la_decay(q.contiguous(), k.contiguous(), v.contiguous(), ld, 1, 1, H, D)
+    out, st2 = ops.la_decay(q, k, v, ld, 1, 1, H, D, out=odd(H * D))
+    assert torch.equal(out, want) and torch.equal(st, st2)
+    assert torch.equal(ops.la_decay_step(q, k, v, ld, st, H, D, out=odd(H * D)), ops.la_decay_step(q, k, v, ld, st2, H, D))
+    x, w = odd(144), ops.fp8_quantize(torch.randn(24, 144, device="cuda").to(dtype), 128)
+    a, b = ops.fp8_quantize(x), ops.fp8_quantize(x.contiguous())
+    assert torch.equal(a.dequantize(), b.dequantize())
+    o = torch.zeros(1, 37, dtype=BF16, device="cuda")[:, :24]
+    r = torch.randn(1, 37, device="cuda").to(BF16)[:, :24]
+    assert torch.equal(ops.gemm_fp8(a, w, residual=r, out=o), ops.gemm_fp8(b, w, residual=r.contiguous()))
