@@ -257,7 +257,8 @@ int sana_la_rope_take_device_status(int* status_out);
  *   lengths [B] int32 on the device, or NULL: sequence b has lengths[b] tokens (clamped to [0, N]); what the
  *   rows behind them hold has no effect, their outputs are zeros, and the state is the one after token lengths[b] - 1 (or prior, or zeros)
  *   workspace: sana_la_decay_workspace_bytes(B, N, H, D, dtype) bytes on the current device (may be 0; < 0: invalid
- *   arguments), 16-byte aligned.
+ *   arguments), 16-byte aligned.  sana_la_decay_plan gives the bytes that a call with (ragged != 0) or without lengths
+ *   needs, which may be fewer, and the number of its kernel launches.
  * State, decays and normalisers are fp32.  Both sides of the bf16 products are bf16, and what was fp32 enters them as a sum
  * of bf16 terms (one: off by 2^-8 of the value at most, two: 2^-17, three: 2^-24):
  *                                     up to 64 tokens     more
@@ -274,6 +275,7 @@ int sana_la_rope_take_device_status(int* status_out);
  * batch names already, leaves the state alone and gives NaN outputs.
  */
 int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype);
+int64_t sana_la_decay_plan(int64_t B, int64_t N, int64_t H, int64_t D, int dtype, int ragged, int* launches);
 int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                   const float* log_decay,
                   const float* prior, const int32_t* lengths, float* state, void* out, int64_t ldo, void* workspace,

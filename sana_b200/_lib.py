@@ -67,6 +67,7 @@ SIGNATURES = {
     "sana_add_f32": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "sana_la_rope_apply": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
     "sana_la_decay_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32]),
+    "sana_la_decay_plan": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32, C.POINTER(C.c_int)]),
     "sana_la_decay": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
                              _i64, _f32, _i32, _f32, _i32, _vp]),
     "sana_la_decay_take_device_status": (_i32, [C.POINTER(C.c_int)]),

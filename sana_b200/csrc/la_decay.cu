@@ -741,11 +741,17 @@ static int ld_check(const char* who, int64_t ldq, int64_t ldk, int64_t ldv, int6
 
 using namespace sana;
 
-extern "C" int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype) {
+extern "C" int64_t sana_la_decay_plan(int64_t B, int64_t N, int64_t H, int64_t D, int dtype, int ragged, int* launches) {
   if (B <= 0 || N <= 0 || N >= ((int64_t)1 << 30) || H <= 0 || !ld_head_dim(D) || (dtype != SANA_BF16 && dtype != SANA_F32)) return -1;
-  int len = 0, nseg = 1, npart[2] = {0, 0};
-  for (int ragged = 0; ragged < 2; ++ragged) LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, ragged != 0, &len, &nseg, &npart[ragged])));
-  return (int64_t)4 * B * (npart[0] > npart[1] ? npart[0] : npart[1]) * H * (D + 1) * D;
+  int len = 0, nseg = 1, npart = 0;
+  LD_DISPATCH(D, (ld_plan<HD>(B, N, H, dtype, ragged != 0, &len, &nseg, &npart)));
+  if (launches) *launches = npart > 0 ? 2 : 1;  // segments are summed by a launch of their own
+  return (int64_t)4 * B * npart * H * (D + 1) * D;
+}
+
+extern "C" int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype) {
+  const int64_t even = sana_la_decay_plan(B, N, H, D, dtype, 0, nullptr), ragged = sana_la_decay_plan(B, N, H, D, dtype, 1, nullptr);
+  return even > ragged ? even : ragged;
 }
 
 extern "C" int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* log_decay,

@@ -928,7 +928,8 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
         _check_out_place("la_decay", out, q, k, v)
     lib = _lib.load()
     state = torch.empty(B, H, D + 1, D, dtype=torch.float32, device=q.device)
-    ws_bytes = lib.sana_la_decay_workspace_bytes(B, N, H, D, dt)
+    launches = C.c_int(0)
+    ws_bytes = lib.sana_la_decay_plan(B, N, H, D, dt, 0 if lens is None else 1, C.byref(launches))
     if ws_bytes < 0:
         raise SanaLibraryError("la_decay: sizes out of range")
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
@@ -937,7 +938,7 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
                                  ldo if ro > 1 else co,
                                  ws.data_ptr() if ws is not None else None, ws_bytes, B, N, H, Hk, D, scale, 1 if relu else 0,
                                  -1.0 if eps is None else eps, dt, _stream_of(dev)), "sana_la_decay")
-    counters.launches += 2 if ws_bytes else 1
+    counters.launches += launches.value
     return out, state
 
 
