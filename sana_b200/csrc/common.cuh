@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/sana_b200.h"
 
 namespace sana {
@@ -37,16 +39,28 @@ int sm_count();  // SMs of the current device (cached per device)
 // kernels (process-wide; set by sana_exchange_set_wait_limit_ns, 2 s unless changed).
 long long exchange_wait_limit_ns();
 
-// One flag per device for set-up that must happen once on every device the process uses
-// (function attributes live in a device's context).  A lost race repeats harmless work.
+// One flag per device for set-up that must happen on every device the process uses (function attributes live in a
+// device's context):  if (auto first = once.first_time()) { set up }  The flag is raised when `first` ends, after the work:
+// a thread that comes meanwhile does the same work again, which is harmless, instead of launching without it.
 struct OncePerDevice {
-  bool done[64] = {};
-  bool first_time() {
+  class Turn {
+   public:
+    explicit Turn(std::atomic<bool>* flag, bool todo) : flag_(flag), todo_(todo) {}
+    Turn(const Turn&) = delete;
+    ~Turn() {
+      if (todo_ && flag_) flag_->store(true, std::memory_order_release);
+    }
+    explicit operator bool() const { return todo_; }
+
+   private:
+    std::atomic<bool>* flag_;
+    bool todo_;
+  };
+  std::atomic<bool> done[64] = {};
+  Turn first_time() {
     int d = 0;
-    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) return true;
-    if (done[d]) return false;
-    done[d] = true;
-    return true;
+    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) return Turn(nullptr, true);
+    return Turn(&done[d], !done[d].load(std::memory_order_acquire));
   }
 };
 

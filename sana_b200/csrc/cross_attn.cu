@@ -252,7 +252,7 @@ static int launch_ca_bf16(const void* q, int64_t ldq, const void* k, const void*
   const int smem_bytes = (CA_BQ + 4 * CA_BK) * (HDP + 8) * 2 + nkc * CA_BK * 4;
   if (smem_bytes > 227 * 1024) return fail(SANA_ERR_UNSUPPORTED, "sana_cross_attention: too many keys (%lld)", (long long)L);
   static OncePerDevice attr_once;
-  if (attr_once.first_time()) {
+  if (auto first = attr_once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(cross_attn_bf16_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(cross_attn)");
   }

@@ -566,7 +566,7 @@ int cross_attn_tc_launch(const void* q, int64_t ldq, const void* k, const void* 
   rc = view(&tmO, out, ldo, N, 32);
   if (rc) return rc;
   static OncePerDevice attr_once;
-  if (attr_once.first_time()) {
+  if (auto first = attr_once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(cross_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, CX_SMEM);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(cross_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, CX_SMEM);

@@ -430,7 +430,7 @@ static int dwconv_glu_impl(const void* u, const void* halo_top, const void* halo
     const int64_t gz = ceil_div(rows, seg);
     SANA_REQUIRE(gy < 65536 && gz < 65536, "sana_dwconv_glu: grid too large");
     static OncePerDevice attr_once;
-    if (attr_once.first_time()) {
+    if (auto first = attr_once.first_time()) {
       cudaError_t e = cudaFuncSetAttribute(dwconv_glu_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DW_SMEM_BYTES);
       if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(dwconv_glu)");
     }

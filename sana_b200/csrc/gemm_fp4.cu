@@ -689,7 +689,7 @@ extern "C" int sana_gemm_nvfp4(const void* Aq, const void* sfa, const float* a_s
       if (rc) return rc;
     }
     static OncePerDevice pair_once;
-    if (pair_once.first_time()) {
+    if (auto first = pair_once.first_time()) {
       cudaError_t e = cudaFuncSetAttribute(gemm_nvfp4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P4_SMEM_BYTES);
       if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_nvfp4_pair)");
     }
@@ -715,7 +715,7 @@ extern "C" int sana_gemm_nvfp4(const void* Aq, const void* sfa, const float* a_s
   rc = make_tmap_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, Wq, N, K / 2, K / 2, F4_BN, 128);
   if (rc) return rc;
   static OncePerDevice attr_once;
-  if (attr_once.first_time()) {
+  if (auto first = attr_once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(gemm_nvfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_nvfp4_tc)");
   }

@@ -922,7 +922,7 @@ static int launch_gemm_fp8(bool pair, const CUtensorMap& tmA, const CUtensorMap&
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   SANA_REQUIRE(tiles < ((int64_t)1 << 30), "sana_gemm_fp8: too many tiles");
   static OncePerDevice once;
-  if (once.first_time()) {
+  if (auto first = once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM_BYTES);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(gemm_fp8_tc_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S8_SMEM_BYTES);

@@ -330,7 +330,7 @@ static int launch_bn(const CUtensorMap& tmA, const void* Wt, int64_t ldw, int64_
     if (rc) return rc;
   }
   static OncePerDevice attr_once;
-  if (attr_once.first_time()) {
+  if (auto first = attr_once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(gemm_bf16_tc_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_bf16_tc)");

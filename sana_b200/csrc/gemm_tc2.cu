@@ -260,7 +260,7 @@ static int launch_pair_bn(const void* A, int64_t lda, const void* Wt, int64_t ld
     tmRes = tmOut;
   }
   static OncePerDevice attr_once;
-  if (attr_once.first_time()) {
+  if (auto first = attr_once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_bf16_tc2)");

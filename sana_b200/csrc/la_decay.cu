@@ -684,7 +684,7 @@ static int launch_decay(LdArgs& a, int64_t B, int dtype, int64_t workspace_bytes
   if (dtype == SANA_BF16) {
     if (a.N >= LD_TC_TOKENS) return launch_decay_tc(a, B, D, st);
     static OncePerDevice once;
-    if (once.first_time()) {
+    if (auto first = once.first_time()) {
       cudaError_t e = cudaFuncSetAttribute(la_decay_short_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ld<D>::BYTES);
       if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(la_decay_short)");
     }

@@ -775,7 +775,7 @@ template <int D, int NT, bool OUT>
 static int lt_launch(const LdMaps& m, const LdArgs& a, int nseg, int64_t B, cudaStream_t st) {
   using T = Lt<D, NT, OUT>;
   static OncePerDevice once;
-  if (once.first_time()) {
+  if (auto first = once.first_time()) {
     cudaError_t e = cudaFuncSetAttribute(la_decay_tc_kernel<D, NT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::BYTES);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(la_decay_tc)");
   }

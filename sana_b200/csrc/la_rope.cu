@@ -629,7 +629,8 @@ struct LrSizes {
 template <int D>
 static int lr_prepare() {
   static OncePerDevice once;
-  if (!once.first_time()) return SANA_OK;
+  auto first = once.first_time();
+  if (!first) return SANA_OK;
   cudaError_t e = cudaFuncSetAttribute(la_rope_apply_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)LrSizes<D>::apply_f32);
   if (e == cudaSuccess)
