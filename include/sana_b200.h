@@ -265,9 +265,9 @@ int sana_la_rope_take_device_status(int* status_out);
  *   state, with q                     two                 one; its key sum two
  *   decayed scores, with v            two                 one (their sum, for the normaliser: fp32)
  *   decayed tokens, in the update     v in three          k in three; two where the state only serves the outputs
- * Bit-reproducible.  An infinity or
- * NaN in v gives NaN in its channel from its token on, one in k or q what the sums make of it; no output before the
- * token is touched.
+ * Bit-reproducible.  No output depends on a later token, whatever that token holds.  An infinity or NaN in v gives NaN in its
+ * channel from its token on (bf16; fp32, and sana_la_decay_step, what the sums make of it), one in k or q what the sums
+ * make of it.
  *
  * sana_la_decay_step: one token of each of B sequences.  q, k, v, out hold B rows; state [pool, H, D+1, D] is updated in
  * place, row b of the batch using entry slots[b] (slots [B] int32 on the device, or NULL for entry b).  A slot of -1
@@ -277,13 +277,11 @@ int sana_la_rope_take_device_status(int* status_out);
 int64_t sana_la_decay_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t D, int dtype);
 int64_t sana_la_decay_plan(int64_t B, int64_t N, int64_t H, int64_t D, int dtype, int ragged, int* launches);
 int sana_la_decay(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                  const float* log_decay,
-                  const float* prior, const int32_t* lengths, float* state, void* out, int64_t ldo, void* workspace,
+                  const float* log_decay, const float* prior, const int32_t* lengths, float* state, void* out, int64_t ldo, void* workspace,
                   int64_t workspace_bytes, int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t D, float scale,
                   int relu, float eps, int dtype, void* stream);
 int sana_la_decay_step(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                  const float* log_decay,
-                       float* state, int64_t pool, const int32_t* slots, void* out, int64_t ldo, int64_t B, int64_t H,
+                       const float* log_decay, float* state, int64_t pool, const int32_t* slots, void* out, int64_t ldo, int64_t B, int64_t H,
                        int64_t Hk, int64_t D, float scale, int relu, float eps, int dtype, void* stream);
 /* Soft-error word of the tcgen05 kernels of sana_la_decay, whose waits are bounded (as sana_la_rope_take_device_status). */
 int sana_la_decay_take_device_status(int* status_out);

@@ -13,13 +13,13 @@
 //
 // bf16, more than 64 tokens: la_decay_tc.cu.  bf16 kernel here: prompts of at most 64 tokens, one chunk, a CTA for one head
 // (narrow heads: several), bound by latency - it starts and ends faster than the tensor-memory kernels' pipeline (64 tokens:
-// 8 x 70 heads of 32 channels 10 us against 16, 8 x 16 heads of 128 14 against 21; 20 heads of 112 12 against 11).  The state lives in the accumulator
-// registers of the warps: warp w owns value channels 16 w .. 16 w + 15 against all key channels.  The accumulator fragment
+// 8 x 70 heads of 32 channels 10 us against 16, 8 x 16 heads of 128 14 against 21; 20 heads of 112 12 against 11).  The
+// state lives in the accumulator registers of the warps: warp w owns value channels 16 w .. 16 w + 15 against all key channels.  The accumulator fragment
 // of S is, register for register, the B operand of S phi(q) (rows of S are the columns of the product), and the transposed
 // fragment of v that multiplies the scores is the A operand of the state update, so the state never moves and v is read
 // from shared memory once.
 // The state stays within a few 2^-24 of fp32: the weighted v is split into three bf16 terms (8 bits each) before the
-// tensor core sees it.  In S phi(q) the state, and before v the scores, enter as two bf16 terms (2^-16): an output of a few
+// tensor core sees it.  In S phi(q) the state, and before v the scores, enter as two bf16 terms (2^-17): an output of a few
 // tokens would feel one rounding of a score as much as its own (a longer sum averages them: la_decay_tc.cu rounds once).
 // The normaliser is summed in fp32 from the unrounded scores.
 // fp32: the chunked form on the CUDA cores.  A sequence is split over CTAs into segments when there are fewer heads than the
@@ -174,215 +174,209 @@ __global__ void __launch_bounds__(Ld<D>::THREADS) la_decay_short_kernel(const Ld
       }
     __syncthreads();
   }
-  {
-    {
-      if (active) {
-        // scores of the 16 x 16 blocks on and below the diagonal, dealt to the warps in turn
-        int id = 0;
-        for (int mi = 0; mi * 16 < nv; ++mi) {
-          for (int ni = 0; ni <= mi; ++ni, ++id) {
-            if (id % WH != wh) continue;
-            float p[2][4] = {};
+  if (active) {
+    // scores of the 16 x 16 blocks on and below the diagonal, dealt to the warps in turn
+    int id = 0;
+    for (int mi = 0; mi * 16 < nv; ++mi) {
+      for (int ni = 0; ni <= mi; ++ni, ++id) {
+        if (id % WH != wh) continue;
+        float p[2][4] = {};
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              uint32_t qa[4], kb[4];
-              ldsm_x4(qa, Qs + mi * 16 * T::ROW + off_rows + kt * 32);
-              ldsm_x4(kb, Ks + ni * 16 * T::ROW + off_cols + kt * 32);
-              if (relu) ld_relu4(qa), ld_relu4(kb);
-              mma_bf16_16816(p[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
-              mma_bf16_16816(p[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
-            }
-            float sum[2] = {0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int d = 16 * (mi - ni) + g + 8 * (e >> 1) - (8 * n + c2 + (e & 1));  // t - s
-                p[n][e] = d >= 0 ? p[n][e] * pow_s[d] : 0.f;
-                sum[e >> 1] += p[n][e];
-              }
-            unsigned char* pr = smem + T::OFF_P + (16 * mi + g) * T::PROW;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              unsigned char* at = pr + 2 * (16 * ni + 8 * n + c2);
-              *reinterpret_cast<uint32_t*>(at) = ld_split(p[n][0], p[n][1]);
-              *reinterpret_cast<uint32_t*>(at + 8 * T::PROW) = ld_split(p[n][2], p[n][3]);
-              *reinterpret_cast<uint32_t*>(at + C * T::PROW) = pack_bf16(p[n][0], p[n][1]);
-              *reinterpret_cast<uint32_t*>(at + (C + 8) * T::PROW) = pack_bf16(p[n][2], p[n][3]);
-            }
-            if (a.normalise) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
-                if (c2 == 0) *reinterpret_cast<float*>(pr + 8 * e * T::PROW + 2 * C + 4 * ni) = sum[e];
-              }
-            }
-          }
+        for (int kt = 0; kt < KT; ++kt) {
+          uint32_t qa[4], kb[4];
+          ldsm_x4(qa, Qs + mi * 16 * T::ROW + off_rows + kt * 32);
+          ldsm_x4(kb, Ks + ni * 16 * T::ROW + off_cols + kt * 32);
+          if (relu) ld_relu4(qa), ld_relu4(kb);
+          mma_bf16_16816(p[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
+          mma_bf16_16816(p[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
         }
-        if (a.normalise) {  // q . key sum, the key sum as two bf16 terms in columns 0 and 1 of the B operand
-          for (int mi = wh; mi * 16 < nv; mi += WH) {
-            float d[4] = {};
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              uint32_t qa[4];
-              ldsm_x4(qa, Qs + mi * 16 * T::ROW + off_rows + kt * 32);
-              if (relu) ld_relu4(qa);
-              uint32_t zb[2];
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float2 z = *reinterpret_cast<const float2*>(z_s + 16 * kt + 8 * e + c2);
-                const uint32_t hi = ld_split(z.x, z.y);
-                zb[e] = g == 0 ? hi : g == 1 ? pack_bf16(z.x, z.y) : 0u;
-              }
-              mma_bf16_16816(d, qa[0], qa[1], qa[2], qa[3], zb[0], zb[1]);
-            }
-            if (c2 == 0) {
-              qz_s[16 * mi + g] = d[0] + d[1];
-              qz_s[16 * mi + g + 8] = d[2] + d[3];
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int d = 16 * (mi - ni) + g + 8 * (e >> 1) - (8 * n + c2 + (e & 1));  // t - s
+            p[n][e] = d >= 0 ? p[n][e] * pow_s[d] : 0.f;
+            sum[e >> 1] += p[n][e];
+          }
+        unsigned char* pr = smem + T::OFF_P + (16 * mi + g) * T::PROW;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          unsigned char* at = pr + 2 * (16 * ni + 8 * n + c2);
+          *reinterpret_cast<uint32_t*>(at) = ld_split(p[n][0], p[n][1]);
+          *reinterpret_cast<uint32_t*>(at + 8 * T::PROW) = ld_split(p[n][2], p[n][3]);
+          *reinterpret_cast<uint32_t*>(at + C * T::PROW) = pack_bf16(p[n][0], p[n][1]);
+          *reinterpret_cast<uint32_t*>(at + (C + 8) * T::PROW) = pack_bf16(p[n][2], p[n][3]);
+        }
+        if (a.normalise) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+            if (c2 == 0) *reinterpret_cast<float*>(pr + 8 * e * T::PROW + 2 * C + 4 * ni) = sum[e];
           }
         }
       }
-      __syncthreads();  // scores and normalisers are there
     }
-    if (!active) return;
-    uint32_t vf[4][4];  // v of the chunk, this warp's 16 channels: [token tile][(s 0-7, ch 0-7), (s 8-15, 0-7), (0-7, 8-15), (8-15, 8-15)]
+    if (a.normalise) {  // q . key sum, the key sum as two bf16 terms in columns 0 and 1 of the B operand
+      for (int mi = wh; mi * 16 < nv; mi += WH) {
+        float d[4] = {};
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) ldsm_x4_t(vf[kt], Vs + kt * 16 * T::ROW + off_rows + wh * 32);
-    {
-      float o[4][2][4] = {};
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {  // S phi(q): key channels 16 kt ..
-        uint32_t hi[2][2], lo[2][2];     // [rows of S 0-7, 8-15 = output column tile][k half]
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = S[2 * kt + e][2 * r], y = S[2 * kt + e][2 * r + 1];
-            hi[r][e] = ld_split(x, y);
-            lo[r][e] = pack_bf16(x, y);
-          }
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
+        for (int kt = 0; kt < KT; ++kt) {
           uint32_t qa[4];
           ldsm_x4(qa, Qs + mi * 16 * T::ROW + off_rows + kt * 32);
           if (relu) ld_relu4(qa);
+          uint32_t zb[2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            mma_bf16_16816(o[mi][r], qa[0], qa[1], qa[2], qa[3], hi[r][0], hi[r][1]);
-            mma_bf16_16816(o[mi][r], qa[0], qa[1], qa[2], qa[3], lo[r][0], lo[r][1]);
+          for (int e = 0; e < 2; ++e) {
+            float2 z = *reinterpret_cast<const float2*>(z_s + 16 * kt + 8 * e + c2);
+            const uint32_t hi = ld_split(z.x, z.y);
+            zb[e] = g == 0 ? hi : g == 1 ? pack_bf16(z.x, z.y) : 0u;
           }
+          mma_bf16_16816(d, qa[0], qa[1], qa[2], qa[3], zb[0], zb[1]);
         }
-      }
-#pragma unroll
-      for (int mi = 0; mi < 4; ++mi) {
-        if (16 * mi >= nv) break;
-        const float f0 = pow_s[16 * mi + g + 1], f1 = pow_s[16 * mi + g + 9];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) o[mi][r][0] *= f0, o[mi][r][1] *= f0, o[mi][r][2] *= f1, o[mi][r][3] *= f1;
-#pragma unroll
-        for (int kt = 0; kt <= mi; ++kt) {
-          uint32_t pa[4];
-#pragma unroll
-          for (int s = 1; s >= 0; --s) {  // the second terms first
-            ldsm_x4(pa, Ps + (s * C + 16 * mi + (lane & 15)) * T::PROW + (lane >> 4) * 16 + kt * 32);
-            mma_bf16_16816(o[mi][0], pa[0], pa[1], pa[2], pa[3], vf[kt][0], vf[kt][1]);
-            mma_bf16_16816(o[mi][1], pa[0], pa[1], pa[2], pa[3], vf[kt][2], vf[kt][3]);
-          }
+        if (c2 == 0) {
+          qz_s[16 * mi + g] = d[0] + d[1];
+          qz_s[16 * mi + g + 8] = d[2] + d[3];
         }
-        float m0 = a.scale, m1 = a.scale;
-        if (a.normalise) {
-          const unsigned char* pr = smem + T::OFF_P + (16 * mi + g) * T::PROW + 2 * C;
-          float d0 = f0 * qz_s[16 * mi + g], d1 = f1 * qz_s[16 * mi + g + 8];
-#pragma unroll
-          for (int ni = 0; ni <= mi; ++ni) {
-            d0 += *reinterpret_cast<const float*>(pr + 4 * ni);
-            d1 += *reinterpret_cast<const float*>(pr + 8 * T::PROW + 4 * ni);
-          }
-          m0 = 1.f / (d0 + a.eps);
-          m1 = 1.f / (d1 + a.eps);
-        }
-        if (odd) {
-          const float nan = __uint_as_float(0x7fffffffu);
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (16 * mi + g + 8 * (e >> 1) >= bad_s[16 * wh + 8 * r + c2 + (e & 1)]) o[mi][r][e] = nan;
-        }
-        // the four lanes of a row group swap so that each holds 16 bytes of one row: lane 0 / 1 row g, channels 0-7 / 8-15,
-        // lane 2 / 3 the same of row g + 8
-        uint32_t w[4] = {pack_bf16(o[mi][0][0] * m0, o[mi][0][1] * m0), pack_bf16(o[mi][1][0] * m0, o[mi][1][1] * m0),
-                         pack_bf16(o[mi][0][2] * m1, o[mi][0][3] * m1), pack_bf16(o[mi][1][2] * m1, o[mi][1][3] * m1)};
-        const int c = lane & 3;
-#pragma unroll
-        for (int s = 1; s < 4; s <<= 1) {  // transpose by exchanging with lane c ^ s
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i & s) continue;
-            const uint32_t give = (c & s) ? w[i] : w[i | s];
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, s);
-            if (c & s) w[i] = got; else w[i | s] = got;
-          }
-        }
-        const int t = 16 * mi + g + 8 * (c >> 1);
-        if (t < nv)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 16 * wh +
-                                    8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    // state update: S = lambda^nv S + (weighted v)^T k.  The tensor core truncates its fp32 sums, so a chunk is summed on
-    // its own, smallest terms first, and joined to the state by one rounded multiply-add.
-    const float whole = pow_s[nv];
-    uint32_t va[4][3][4], wa[4][2];  // three terms of the weighted v (A operand); terms of the weights in rows 0..2
+  }
+  __syncthreads();  // scores and normalisers are there
+  if (!active) return;
+  uint32_t vf[4][4];  // v of the chunk, this warp's 16 channels: [token tile][(s 0-7, ch 0-7), (s 8-15, 0-7), (0-7, 8-15), (8-15, 8-15)]
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+  for (int kt = 0; kt < 4; ++kt) ldsm_x4_t(vf[kt], Vs + kt * 16 * T::ROW + off_rows + wh * 32);
+  float o[4][2][4] = {};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // tokens 16 kt + 8 e + c2, + 1
-        const int left = nv - 1 - (16 * kt + 8 * e + c2);
-        float w0 = left >= 0 ? pow_s[left] : 0.f, w1 = left >= 1 ? pow_s[left - 1] : 0.f;
+  for (int kt = 0; kt < KT; ++kt) {  // S phi(q): key channels 16 kt ..
+    uint32_t hi[2][2], lo[2][2];     // [rows of S 0-7, 8-15 = output column tile][k half]
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {  // channels 0-7, 8-15: fragment register vf[2 r + e], A register 2 e + r
-          float x = bf16_lo(vf[kt][2 * r + e]) * w0, y = bf16_hi(vf[kt][2 * r + e]) * w1;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int s = 0; s < 3; ++s) va[kt][s][2 * e + r] = ld_split(x, y);
-        }
-        const uint32_t t0 = ld_split(w0, w1), t1 = ld_split(w0, w1), t2 = ld_split(w0, w1);
-        wa[kt][e] = g == 0 ? t0 : g == 1 ? t1 : g == 2 ? t2 : 0u;
+      for (int e = 0; e < 2; ++e) {
+        float x = S[2 * kt + e][2 * r], y = S[2 * kt + e][2 * r + 1];
+        hi[r][e] = ld_split(x, y);
+        lo[r][e] = pack_bf16(x, y);
       }
 #pragma unroll
-    for (int n = 0; n < KT; ++n) {
-      uint32_t kb[4][4];  // k[tokens][16 n ..] as the B operand of two column tiles
-      float d[2][4] = {};
+    for (int mi = 0; mi < 4; ++mi) {
+      uint32_t qa[4];
+      ldsm_x4(qa, Qs + mi * 16 * T::ROW + off_rows + kt * 32);
+      if (relu) ld_relu4(qa);
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        ldsm_x4_t(kb[kt], Ks + kt * 16 * T::ROW + off_rows + n * 32);
-        if (relu) ld_relu4(kb[kt]);
+      for (int r = 0; r < 2; ++r) {
+        mma_bf16_16816(o[mi][r], qa[0], qa[1], qa[2], qa[3], hi[r][0], hi[r][1]);
+        mma_bf16_16816(o[mi][r], qa[0], qa[1], qa[2], qa[3], lo[r][0], lo[r][1]);
       }
+    }
+  }
 #pragma unroll
-      for (int s = 2; s >= 0; --s)
+  for (int mi = 0; mi < 4; ++mi) {
+    if (16 * mi >= nv) break;
+    const float f0 = pow_s[16 * mi + g + 1], f1 = pow_s[16 * mi + g + 9];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          mma_bf16_16816(d[0], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][0], kb[kt][1]);
-          mma_bf16_16816(d[1], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][2], kb[kt][3]);
-        }
+    for (int r = 0; r < 2; ++r) o[mi][r][0] *= f0, o[mi][r][1] *= f0, o[mi][r][2] *= f1, o[mi][r][3] *= f1;
+#pragma unroll
+    for (int kt = 0; kt <= mi; ++kt) {
+      uint32_t pa[4];
+#pragma unroll
+      for (int s = 1; s >= 0; --s) {  // the second terms first
+        ldsm_x4(pa, Ps + (s * C + 16 * mi + (lane & 15)) * T::PROW + (lane >> 4) * 16 + kt * 32);
+        mma_bf16_16816(o[mi][0], pa[0], pa[1], pa[2], pa[3], vf[kt][0], vf[kt][1]);
+        mma_bf16_16816(o[mi][1], pa[0], pa[1], pa[2], pa[3], vf[kt][2], vf[kt][3]);
+      }
+    }
+    float m0 = a.scale, m1 = a.scale;
+    if (a.normalise) {
+      const unsigned char* pr = smem + T::OFF_P + (16 * mi + g) * T::PROW + 2 * C;
+      float d0 = f0 * qz_s[16 * mi + g], d1 = f1 * qz_s[16 * mi + g + 8];
+#pragma unroll
+      for (int ni = 0; ni <= mi; ++ni) {
+        d0 += *reinterpret_cast<const float*>(pr + 4 * ni);
+        d1 += *reinterpret_cast<const float*>(pr + 8 * T::PROW + 4 * ni);
+      }
+      m0 = 1.f / (d0 + a.eps);
+      m1 = 1.f / (d1 + a.eps);
+    }
+    if (odd) {
+      const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[2 * n + r][e] = fmaf(whole, S[2 * n + r][e], d[r][e]);
-      if (n == wh) {
-        float z[2][4] = {};
+        for (int e = 0; e < 4; ++e)
+          if (16 * mi + g + 8 * (e >> 1) >= bad_s[16 * wh + 8 * r + c2 + (e & 1)]) o[mi][r][e] = nan;
+    }
+    // the four lanes of a row group swap so that each holds 16 bytes of one row: lane 0 / 1 row g, channels 0-7 / 8-15,
+    // lane 2 / 3 the same of row g + 8
+    uint32_t w[4] = {pack_bf16(o[mi][0][0] * m0, o[mi][0][1] * m0), pack_bf16(o[mi][1][0] * m0, o[mi][1][1] * m0),
+                     pack_bf16(o[mi][0][2] * m1, o[mi][0][3] * m1), pack_bf16(o[mi][1][2] * m1, o[mi][1][3] * m1)};
+    const int c = lane & 3;
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          mma_bf16_16816(z[0], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][0], kb[kt][1]);
-          mma_bf16_16816(z[1], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][2], kb[kt][3]);
-        }
+    for (int s = 1; s < 4; s <<= 1) {  // transpose by exchanging with lane c ^ s
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) zacc[r][e] = fmaf(whole, zacc[r][e], z[r][e]);
+      for (int i = 0; i < 4; ++i) {
+        if (i & s) continue;
+        const uint32_t give = (c & s) ? w[i] : w[i | s];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, s);
+        if (c & s) w[i] = got; else w[i | s] = got;
       }
+    }
+    const int t = 16 * mi + g + 8 * (c >> 1);
+    if (t < nv)
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (row0 + t) * a.ldo + (int64_t)h * D + 16 * wh +
+                                8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // state update: S = lambda^nv S + (weighted v)^T k.  The tensor core truncates its fp32 sums, so a chunk is summed on
+  // its own, smallest terms first, and joined to the state by one rounded multiply-add.
+  const float whole = pow_s[nv];
+  uint32_t va[4][3][4], wa[4][2];  // three terms of the weighted v (A operand); terms of the weights in rows 0..2
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // tokens 16 kt + 8 e + c2, + 1
+      const int left = nv - 1 - (16 * kt + 8 * e + c2);
+      float w0 = left >= 0 ? pow_s[left] : 0.f, w1 = left >= 1 ? pow_s[left - 1] : 0.f;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {  // channels 0-7, 8-15: fragment register vf[2 r + e], A register 2 e + r
+        float x = bf16_lo(vf[kt][2 * r + e]) * w0, y = bf16_hi(vf[kt][2 * r + e]) * w1;
+#pragma unroll
+        for (int s = 0; s < 3; ++s) va[kt][s][2 * e + r] = ld_split(x, y);
+      }
+      const uint32_t t0 = ld_split(w0, w1), t1 = ld_split(w0, w1), t2 = ld_split(w0, w1);
+      wa[kt][e] = g == 0 ? t0 : g == 1 ? t1 : g == 2 ? t2 : 0u;
+    }
+#pragma unroll
+  for (int n = 0; n < KT; ++n) {
+    uint32_t kb[4][4];  // k[tokens][16 n ..] as the B operand of two column tiles
+    float d[2][4] = {};
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      ldsm_x4_t(kb[kt], Ks + kt * 16 * T::ROW + off_rows + n * 32);
+      if (relu) ld_relu4(kb[kt]);
+    }
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        mma_bf16_16816(d[0], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][0], kb[kt][1]);
+        mma_bf16_16816(d[1], va[kt][s][0], va[kt][s][1], va[kt][s][2], va[kt][s][3], kb[kt][2], kb[kt][3]);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[2 * n + r][e] = fmaf(whole, S[2 * n + r][e], d[r][e]);
+    if (n == wh) {
+      float z[2][4] = {};
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        mma_bf16_16816(z[0], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][0], kb[kt][1]);
+        mma_bf16_16816(z[1], wa[kt][0], 0u, wa[kt][1], 0u, kb[kt][2], kb[kt][3]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) zacc[r][e] = fmaf(whole, zacc[r][e], z[r][e]);
     }
   }
   if (odd) {

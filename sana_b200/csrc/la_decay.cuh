@@ -36,8 +36,8 @@ __device__ __forceinline__ uint32_t ld_split(float& a, float& b) {
   return p;
 }
 
-// Split of a sequence into token segments (a multiple of `chunk` tokens each): minimises
-// waves x (chunks of a segment + overhead); more than one segment costs a first pass over k and v.
+// Split of a sequence into nseg token segments of seg_len tokens (whole chunks; the last may be shorter).  The rules that
+// choose it: ld_tc_plan, and ld_plan for fp32.
 struct LdPlan {
   int seg_len, nseg;
 };

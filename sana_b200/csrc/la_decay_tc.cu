@@ -18,15 +18,17 @@
 // keys, apply ReLU in place and put the ones column back beside v; one warp issues the products, one the copies.
 // The weighted k is split into NT bf16 terms: 3 where the state leaves the kernel (2^-24; the truncation of a chunk's 24
 // products adds up to 2e-6 where everything has one sign and nothing decays, 3e-7 otherwise), 2 where it only serves the
-// outputs (2^-16, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
-// rows of one product, and the state warps add them; an instruction costs 42 + N / 2 cycles whatever part of its rows
-// is used.  All waits are bounded.
+// outputs (2^-17, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
+// rows of one product, and the state warps add them: an instruction costs the same (elect_one) whatever part of its rows
+// is used.  The decayed scores enter O2, and the state's value channels O1, as one bf16 term, the carried key sum as two: with
+// the output's own rounding the outputs are off by 2.2e-3 in norm, where that rounding alone gives 1.7e-3 (a second term
+// of the scores, as la_decay.cu takes for its one chunk, would double O2).  All waits are bounded.
 //
 // Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
-// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 229-240 us (2.5 TB/s; 90); 4 x up to 4096, 16 heads of 64 over 8
-// of k and v 68-91.  What bounds it is the length of a chunk's chain - copy, transform, products, join, state operand,
-// products, output, each behind a barrier and with one warp per scheduler for each role: the tensor pipe is busy 17-22 % of
-// the time and DRAM 25-38 %.  Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per
+// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 246-254 us (2.4 TB/s; 90); 8 x 4096 tokens, 16 heads of 128 281 us
+// (two launches; 83); 4 x up to 4096, 16 heads of 64 over 8 of k and v 60-81.  What bounds it is the length of a chunk's
+// chain - copy, transform, products, join, state operand, products, output, each behind a barrier and with one warp per
+// scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.  Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per
 // SM overlap theirs; wide heads fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles
 // that poll several barriers in turn were tried and were slower.
 #include "la_decay.cuh"
@@ -272,8 +274,8 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
     // Row j of the state operand, 8 value channels to a 16-byte piece.  The value channels enter as one bf16 term (2^-8 of each
     // at most, of either sign, summed over D key channels): a second one would double these products and their operand, which
-    // shared memory has no room for next to the second v tile.  The key sum, whose error all channels of an output would share,
-    // enters as two (2^-17): the second takes a column of the padding.
+    // shared memory has no room for beside the second v tile of wide heads.  The key sum, whose error all channels of an
+    // output would share, enters as two (2^-17): the second takes a column of the padding.
     auto key_sum = [](float z) -> uint32_t { return pack_bf16(z, z - __bfloat162float(__float2bfloat16_rn(z))); };
     auto write_operand = [&]() {
       if constexpr (T::STACK) {
@@ -813,7 +815,7 @@ static int lt_run(const LdArgs& a, int64_t B, cudaStream_t st) {
 // [0, N]: CTAs behind the end of a sequence leave at once, (segments + 1) / 2 of a sequence's have work, and these fill one
 // another's gaps, so the waves are not rounded up.  Its split replaces the first one only where it promises at least 15 %,
 // since sequences that all reach N lose by it: 4 x 4096, 16 heads of 64, four segments against two, lengths spread 68 us
-// against 94, one long sequence 57 against 94, all full 109 against 96.
+// against 94, one long sequence 57-60 against 94, all full 109-112 against 96-99.
 LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, bool ragged, int* npart) {
   const int64_t units = B * H, slots = (int64_t)sm_count() * (D <= 32 ? 2 : 1), chunks = ceil_div(N, LT_C);
   auto segment = [&](int64_t len, int64_t real) -> int64_t {  // tenths of a chunk

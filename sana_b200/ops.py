@@ -906,7 +906,8 @@ def la_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch
 
     q [B*N, H*D] and k, v [B*N, Hk*D] views (column blocks of a projection), H a multiple of Hk; log_decay fp32 [H], not
     positive; prior fp32 [B, H, D+1, D], the state carried in; lengths int32 [B] for a padded batch (rows behind a
-    sequence give zeros); out may be q itself, and must not overlap q, k or v otherwise.  Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
+    sequence give zeros); out may be q itself, and must not overlap q, k or v otherwise.
+    Returns (out [B*N, H*D], state fp32 [B, H, D+1, D])."""
     dev = _device_of("la_decay", q, k, v, log_decay, prior, lengths, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):

@@ -63,8 +63,9 @@ def pack_nvfp4_weights(model: nn.Module) -> Dict[str, torch.Tensor]:
 def load_nvfp4_weights(model: nn.Module, pack: Dict[str, torch.Tensor], enable: bool = True) -> int:
     """Installs the packed weights on the matching modules of ``model`` (moved to each module's
     device) so that their NVFP4 projections use them instead of quantising the bf16 weights, and
-    (``enable``) switches those modules to NVFP4 (which replaces the 8-bit setting).  Every NVFP4-capable projection of the model must
-    be in the pack with the right shape.  Returns the number of projections installed."""
+    (``enable``) switches those modules to NVFP4, which replaces the 8-bit setting.  Every NVFP4-capable
+    projection of the model must be in the pack with the right shape.  Returns the number of
+    projections installed."""
     n = 0
     for name, module in model.named_modules():
         for key, w in _projections(module):
