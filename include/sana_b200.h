@@ -263,7 +263,8 @@ int sana_la_rope_take_device_status(int* status_out);
  * of bf16 terms (one: off by 2^-8 of the value at most, two: 2^-17, three: 2^-24):
  *                                     up to 64 tokens     more
  *   state, with q                     two                 one; its key sum two
- *   decayed scores, with v            two                 one (their sum, for the normaliser: fp32)
+ *   decayed scores, with v            two                 two; D = 128: one for tokens 64 .. 127 of each 128
+ *   their sum, for the normaliser     fp32                fp32
  *   decayed tokens, in the update     v in three          k in three; two where the state only serves the outputs
  * Bit-reproducible.  No output depends on a later token, whatever that token holds.  An infinity or NaN in v gives NaN in its
  * channel from its token on (bf16; fp32, and sana_la_decay_step, what the sums make of it), one in k or q what the sums

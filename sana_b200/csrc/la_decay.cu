@@ -14,14 +14,13 @@
 // bf16, more than 64 tokens: la_decay_tc.cu.  bf16 kernel here: prompts of at most 64 tokens, one chunk, a CTA for one head
 // (narrow heads: several), bound by latency - it starts and ends faster than the tensor-memory kernels' pipeline (64 tokens:
 // 8 x 70 heads of 32 channels 10 us against 16, 8 x 16 heads of 128 14 against 21; 20 heads of 112 12 against 11).  The
-// state lives in the accumulator registers of the warps: warp w owns value channels 16 w .. 16 w + 15 against all key channels.  The accumulator fragment
-// of S is, register for register, the B operand of S phi(q) (rows of S are the columns of the product), and the transposed
-// fragment of v that multiplies the scores is the A operand of the state update, so the state never moves and v is read
-// from shared memory once.
+// state lives in the accumulator registers of the warps: warp w owns value channels 16 w .. 16 w + 15 against all key
+// channels.  The accumulator fragment of S is, register for register, the B operand of S phi(q) (rows of S are the columns
+// of the product), and the transposed fragment of v that multiplies the scores is the A operand of the state update, so the
+// state never moves and v is read from shared memory once.
 // The state stays within a few 2^-24 of fp32: the weighted v is split into three bf16 terms (8 bits each) before the
 // tensor core sees it.  In S phi(q) the state, and before v the scores, enter as two bf16 terms (2^-17): an output of a few
-// tokens would feel one rounding of a score as much as its own (a longer sum averages them: la_decay_tc.cu rounds once).
-// The normaliser is summed in fp32 from the unrounded scores.
+// tokens would feel one rounding of a score as much as its own.  The normaliser is summed in fp32 from the unrounded scores.
 // fp32: the chunked form on the CUDA cores.  A sequence is split over CTAs into segments when there are fewer heads than the
 // GPU has room for: a first launch computes what each segment adds to the state, and each CTA of the second combines those
 // of the segments before its own, in order (nothing depends on the order in which CTAs run).

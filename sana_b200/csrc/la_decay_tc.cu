@@ -5,7 +5,7 @@
 //
 //   scores  SC  = phi(Q) phi(K)^T                     M = 128 queries, N = 128 keys, K = D
 //   inter   O1  = phi(Q) S^T                          N = D + 16, K = D          row t is scaled by lambda^(t+1) at the end
-//   intra   O2  = (SC * lambda^(t-s), s <= t) V1      N = D + 16, K = 128        A operand in tensor memory, bf16
+//   intra   O2  = (SC * lambda^(t-s), s <= t) V       N = D, K = 128             A operand in tensor memory, two bf16 terms
 //   state   dS^T = (w K)^T V1                         M = D key channels, N = D + 16, K = 128 tokens
 //
 // Every tile is [64-channel block][row][128 bytes], 128-byte swizzled, which serves as a K-major operand (rows = M or N)
@@ -20,9 +20,9 @@
 // products adds up to 2e-6 where everything has one sign and nothing decays, 3e-7 otherwise), 2 where it only serves the
 // outputs (2^-17, below their own rounding).  Up to 32 channels the terms stand side by side in the 128
 // rows of one product, and the state warps add them: an instruction costs the same (elect_one) whatever part of its rows
-// is used.  The decayed scores enter O2, and the state's value channels O1, as one bf16 term, the carried key sum as two: with
-// the output's own rounding the outputs are off by 2.2e-3 in norm, where that rounding alone gives 1.7e-3 (a second term
-// of the scores, as la_decay.cu takes for its one chunk, would double O2).  All waits are bounded.
+// is used.  The decayed scores enter O2 as two bf16 terms (2^-17; heads of 128 channels: the last 64 keys of a chunk as
+// one, 2^-8), which costs 1-3 % of the time: an output of a few tokens would feel one rounding of a score as much as its
+// own.  The carried key sum enters O1 as two terms, the state's value channels as one (write_operand).  All waits are bounded.
 //
 // Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
 // rate would allow 45); 8 x 4096 tokens, 70 heads of 32 246-254 us (2.4 TB/s; 90); 8 x 4096 tokens, 16 heads of 128 281 us
@@ -82,6 +82,10 @@ struct Lt {
   // second half and the next chunk's scores wait until it has been read.
   static constexpr bool ALIAS = 128 + 2 * NV + D > 512;
   static constexpr int COL_SC = 0, COL_O2 = ALIAS ? 96 : 128;
+  // The decayed scores of 32 keys go over their fp32 scores, which have been read: 16 columns of bf16 pairs, and 16 of what
+  // that rounding left.  Where O2 starts at 96, the last 64 keys have room for the first term only.
+  __host__ __device__ static constexpr bool two_terms(int blk) { return !ALIAS || blk < 2; }
+  __host__ __device__ static constexpr int pair_col(int blk) { return COL_SC + (two_terms(blk) ? 32 * blk : 64 + 16 * (blk - 2)); }
   static constexpr int COL_O1 = COL_O2 + D;
   static constexpr int COL_DS = OUT ? COL_O1 + NV : 0;
   static constexpr int COLS = COL_DS + NV;
@@ -460,12 +464,18 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           if (!lt_wait(scready + 8 * half, (uint32_t)(c & 1), abort_flag, 4)) { ok = false; break; }
           tcgen05_fence_after();
 #pragma unroll 1
-          for (int q = 0; q < 2; ++q) {  // keys 32 blk .. + 31; the bf16 pairs go over scores that have been read
+          for (int q = 0; q < 2; ++q) {  // keys 32 blk .. + 31
             const int blk = 2 * half + q;
-            uint32_t p[16];
+            uint32_t p[16], r[16];  // the first terms, the second ones
+            auto split = [&](int e, const float2 v) {
+              sum = __fadd2_rn(sum, v);
+              p[e] = pack_bf16(v.x, v.y);
+              const float2 left = __fadd2_rn(v, make_float2(-bf16_lo(p[e]), -bf16_hi(p[e])));
+              r[e] = pack_bf16(left.x, left.y);
+            };
             if (blk > w) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) p[e] = 0u;
+              for (int e = 0; e < 16; ++e) p[e] = r[e] = 0u;
             } else {
               uint32_t x[32];
               tmem_ld_32x32(sc + (uint32_t)(32 * blk), x);
@@ -475,22 +485,20 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                   const float2 d = __fmul2_rn(make_float2(f, f), *reinterpret_cast<const float2*>(rev_s + 2 * e));
-                  const float2 v = __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), d);
-                  sum = __fadd2_rn(sum, v);
-                  p[e] = pack_bf16(v.x, v.y);
+                  split(e, __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), d));
                 }
               } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {  // selected, not multiplied by the table's zero: a later token may be NaN
-                  const float2 v = __fmul2_rn(make_float2(lane >= 2 * e ? __uint_as_float(x[2 * e]) : 0.f,
-                                                          lane >= 2 * e + 1 ? __uint_as_float(x[2 * e + 1]) : 0.f),
-                                              make_float2(mine[-2 * e], mine[-2 * e - 1]));
-                  sum = __fadd2_rn(sum, v);
-                  p[e] = pack_bf16(v.x, v.y);
+                  split(e, __fmul2_rn(make_float2(lane >= 2 * e ? __uint_as_float(x[2 * e]) : 0.f,
+                                                  lane >= 2 * e + 1 ? __uint_as_float(x[2 * e + 1]) : 0.f),
+                                      make_float2(mine[-2 * e], mine[-2 * e - 1])));
                 }
               }
             }
-            lt_st16(sc + (uint32_t)(64 * half + 16 * q), p);
+            const uint32_t at = sc + (uint32_t)(T::pair_col(blk) - T::COL_SC);
+            lt_st16(at, p);
+            if (T::two_terms(blk)) lt_st16(at + 16, r);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           if (half == 1 && a.normalise) rs[(c & 1) * C] = sum.x + sum.y;
@@ -692,9 +700,12 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           if (!T::ALIAS || half == 1) {
             if (elect_one()) {
 #pragma unroll 1
-              for (int k = T::ALIAS ? 0 : 4 * half; k < 4 * half + 4; ++k)
-                lt_mma_ts(tmem + T::COL_O2, tmem + T::COL_SC + 64u * (k >> 2) + 8u * (k & 3), vdesc + (uint64_t)(128 * k), T::ID_O2,
-                          k != 0 ? 1u : 0u);
+              for (int k = T::ALIAS ? 0 : 4 * half; k < 4 * half + 4; ++k) {
+                const uint32_t at = tmem + (uint32_t)T::pair_col(k >> 1) + 8u * (k & 1);
+                const bool two = T::two_terms(k >> 1);
+                if (two) lt_mma_ts(tmem + T::COL_O2, at + 16u, vdesc + (uint64_t)(128 * k), T::ID_O2, k != 0 ? 1u : 0u);
+                lt_mma_ts(tmem + T::COL_O2, at, vdesc + (uint64_t)(128 * k), T::ID_O2, k != 0 || two ? 1u : 0u);
+              }
               if (half == 1) {
                 umma_commit(vempty + 8 * (c % T::VBUF));
                 umma_commit(oready);
