@@ -262,7 +262,7 @@ int sana_la_rope_take_device_status(int* status_out);
  * State, decays and normalisers are fp32.  Both sides of the bf16 products are bf16, and what was fp32 enters them as a sum
  * of bf16 terms (one: off by 2^-8 of the value at most, two: 2^-17, three: 2^-24):
  *                                     up to 64 tokens     more
- *   state, with q                     two                 one; its key sum two
+ *   state, with q                     two                 two for D = 16, 48 and 64, else one; its key sum two
  *   decayed scores, with v            two                 two; D = 128: one for tokens 64 .. 127 of each 128
  *   their sum, for the normaliser     fp32                fp32
  *   decayed tokens, in the update     v in three          k in three; two where the state only serves the outputs

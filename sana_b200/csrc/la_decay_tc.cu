@@ -22,15 +22,17 @@
 // rows of one product, and the state warps add them: an instruction costs the same (elect_one) whatever part of its rows
 // is used.  The decayed scores enter O2 as two bf16 terms (2^-17; heads of 128 channels: the last 64 keys of a chunk as
 // one, 2^-8), which costs 1-3 % of the time: an output of a few tokens would feel one rounding of a score as much as its
-// own.  The carried key sum enters O1 as two terms, the state's value channels as one (write_operand).  All waits are bounded.
+// own.  The carried key sum enters O1 as two terms, the state's value channels as two or one (write_operand).  All waits
+// are bounded.
 //
-// Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 158 us (1.86 TB/s of q, k, v, out; the copy
-// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 246-254 us (2.4 TB/s; 90); 8 x 4096 tokens, 16 heads of 128 281 us
-// (two launches; 83); 4 x up to 4096, 16 heads of 64 over 8 of k and v 60-81.  What bounds it is the length of a chunk's
+// Measured (L2 flushed before each run): 20 heads of 112 channels, 16 384 tokens 159 us (1.85 TB/s of q, k, v, out; the copy
+// rate would allow 45); 8 x 4096 tokens, 70 heads of 32 246-254 us (2.4 TB/s; 90); 8 x 4096 tokens, 16 heads of 128 288 us
+// (two launches; 83); 4 x up to 4096, 16 heads of 64 over 8 of k and v 63-86.  What bounds it is the length of a chunk's
 // chain - copy, transform, products, join, state operand, products, output, each behind a barrier and with one warp per
-// scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.  Chunks of 128 halve the number of chains that 64 would have, and two CTAs of narrow heads per
-// SM overlap theirs; wide heads fill shared memory alone.  Single-lane waits (half the speed of converged ones) and roles
-// that poll several barriers in turn were tried and were slower.
+// scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.  Chunks of 128 halve the number of
+// chains that 64 would have, and two CTAs of narrow heads per SM overlap theirs; wide heads fill shared memory alone.
+// Single-lane waits (half the speed of converged ones) and roles that poll several barriers in turn were tried and were
+// slower.
 #include "la_decay.cuh"
 
 namespace sana {
@@ -61,12 +63,16 @@ struct Lt {
   // a second v tile hides the latency of its load behind the products that still need the first; then one for q
   static constexpr int VBUF = ONE_EACH + VTILE <= LIMIT ? 2 : 1;
   static constexpr int QBUF = OUT && ONE_EACH + (VBUF - 1) * VTILE + KTILE <= LIMIT ? 2 : 1;
+  // Terms of the state operand: a second one where there is room for it beside these (16, 48 and 64 channels).  With no decay
+  // to speak of it takes the outputs' error from 2.2e-3 to 1.7e-3, and costs 2 % (16 channels), 11 % (8 x 4096 tokens, 40
+  // heads of 48: 336 -> 373 us), 5-9 % (4 x up to 4096, 16 heads of 64).
+  static constexpr int ST = OUT && ONE_EACH + (VBUF - 1) * VTILE + (QBUF - 1) * KTILE + VB * STATE_BLK <= LIMIT ? 2 : 1;
   static constexpr int OFF_W = 0;                        // weighted k (followed by v: with one block of 64 channels, rows
   static constexpr int OFF_V = OFF_W + WTILE;            // 64 .. 127 of the product read there and are not used)
   static constexpr int OFF_K = OFF_V + VBUF * VTILE;
   static constexpr int OFF_Q = OFF_K + KTILE;
   static constexpr int OFF_S = OFF_Q + (OUT ? QBUF * KTILE : 0);
-  static constexpr int OFF_X = OFF_S + (OUT ? VB * STATE_BLK : 0);
+  static constexpr int OFF_X = OFF_S + (OUT ? ST * VB * STATE_BLK : 0);
   static constexpr int OFF_POW = OFF_X + X_BYTES;        // powers behind 32 zeros
   static constexpr int OFF_RS = OFF_POW + 4 * (32 + LT_C + 2 + 32);  // row sums of the scores, [2][128]
   static constexpr int OFF_BAR = OFF_RS + (OUT ? 4 * 2 * LT_C : 0);
@@ -276,32 +282,49 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           if (held(i)) dst[row_of(i) * D + sj] = fmaf(f, S[i], n_end > n_begin ? __ldg(src + row_of(i) * D + sj) : 0.f);
       }
     }
-    // Row j of the state operand, 8 value channels to a 16-byte piece.  The value channels enter as one bf16 term (2^-8 of each
-    // at most, of either sign, summed over D key channels): a second one would double these products and their operand, which
-    // shared memory has no room for beside the second v tile of wide heads.  The key sum, whose error all channels of an
-    // output would share, enters as two (2^-17): the second takes a column of the padding.
+    // Row j of the state operand, 8 value channels to a 16-byte piece.  The value channels enter as two bf16 terms (2^-17) where
+    // shared memory has room for a second operand, else as one (2^-8 of each at most, of either
+    // sign, summed over D key channels).  The key sum, whose error all channels of an output would share, always enters
+    // as two: the second takes a column of the padding.
     auto key_sum = [](float z) -> uint32_t { return pack_bf16(z, z - __bfloat162float(__float2bfloat16_rn(z))); };
+    auto left2 = [](float a, float b, uint32_t w) -> uint32_t {
+      const float2 d = __fadd2_rn(make_float2(a, b), make_float2(-bf16_lo(w), -bf16_hi(w)));
+      return pack_bf16(d.x, d.y);
+    };
     auto write_operand = [&]() {
       if constexpr (T::STACK) {
         unsigned char* row = smem + T::OFF_S + lane * 128;
-        auto put = [&](int c, const uint4& w) { *reinterpret_cast<uint4*>(row + ((c ^ (lane & 7)) << 4)) = w; };  // c < 8
-        if (lane < D && 8 * warp < D)
-          put(warp, make_uint4(pack_bf16(S[0], S[1]), pack_bf16(S[2], S[3]), pack_bf16(S[4], S[5]), pack_bf16(S[6], S[7])));
+        auto put = [&](int c, const uint4& w, int term = 0) {  // c < 8
+          *reinterpret_cast<uint4*>(row + term * T::VB * T::STATE_BLK + ((c ^ (lane & 7)) << 4)) = w;
+        };
+        if (lane < D && 8 * warp < D) {
+          const uint4 w = make_uint4(pack_bf16(S[0], S[1]), pack_bf16(S[2], S[3]), pack_bf16(S[4], S[5]), pack_bf16(S[6], S[7]));
+          put(warp, w);
+          if (T::ST == 2)
+            put(warp, make_uint4(left2(S[0], S[1], w.x), left2(S[2], S[3], w.y), left2(S[4], S[5], w.z), left2(S[6], S[7], w.w)), 1);
+        }
         if (lane < D && warp == 3) {
           put(D / 8, make_uint4(key_sum(S[8]), 0u, 0u, 0u));
           put(D / 8 + 1, make_uint4(0u, 0u, 0u, 0u));
+          if (T::ST == 2) {
+            put(D / 8, make_uint4(0u, 0u, 0u, 0u), 1);
+            put(D / 8 + 1, make_uint4(0u, 0u, 0u, 0u), 1);
+          }
         }
       } else if (jin) {
         unsigned char* row = smem + T::OFF_S + j * 128;
 #pragma unroll
         for (int c = 0; c < NV / 8; ++c) {
-          uint32_t w[4];
+          uint32_t w[4], r[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 8 * c + 2 * e;
             w[e] = i < D ? pack_bf16(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0]) : i == D ? key_sum(S[NS - 1]) : 0u;
+            r[e] = i < D ? left2(S[i < D ? i : 0], S[i + 1 < D ? i + 1 : 0], w[e]) : 0u;
           }
-          *reinterpret_cast<uint4*>(row + (c >> 3) * T::STATE_BLK + (((c & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          unsigned char* at = row + (c >> 3) * T::STATE_BLK + (((c & 7) ^ (j & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (T::ST == 2) *reinterpret_cast<uint4*>(at + T::VB * T::STATE_BLK) = make_uint4(r[0], r[1], r[2], r[3]);
         }
       }
       fence_proxy_async_smem();
@@ -633,7 +656,6 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if constexpr (T::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 8 + LW) {  // the whole warp waits, one elected lane issues
       const uint32_t Wu = sm + T::OFF_W, Vu = sm + T::OFF_V, Ku = sm + T::OFF_K, Qu = sm + T::OFF_Q, Su = sm + T::OFF_S;
-      const uint64_t sdesc = lt_desc_mn(Su, T::STATE_BLK);
       auto wait = [&](uint32_t bb, uint32_t parity, int code) -> bool {
         return lt_wait(bb, parity, abort_flag, code);
       };
@@ -683,9 +705,13 @@ la_decay_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (elect_one()) {
           const uint32_t Qc = qtile(c);
 #pragma unroll 1
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
-                      T::ID_O1, k != 0 ? 1u : 0u);
+          for (int s = T::ST - 1; s >= 0; --s) {  // smallest term first
+            const uint64_t sdesc = lt_desc_mn(Su + s * T::VB * T::STATE_BLK, T::STATE_BLK);
+#pragma unroll 1
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16(tmem + T::COL_O1, make_smem_desc(Qc + (k >> 2) * LT_BLK) + (uint64_t)(2 * (k & 3)), sdesc + (uint64_t)(128 * k),
+                        T::ID_O1, (s != T::ST - 1 || k != 0) ? 1u : 0u);
+          }
           umma_commit(qempty + 8 * (c % T::QBUF));
           umma_commit(sopread);
         }
@@ -825,8 +851,8 @@ static int lt_run(const LdArgs& a, int64_t B, cudaStream_t st) {
 // Cost of a split = waves of CTAs x the time of a segment.  A padded batch is taken to hold lengths spread evenly over
 // [0, N]: CTAs behind the end of a sequence leave at once, (segments + 1) / 2 of a sequence's have work, and these fill one
 // another's gaps, so the waves are not rounded up.  Its split replaces the first one only where it promises at least 15 %,
-// since sequences that all reach N lose by it: 4 x 4096, 16 heads of 64, four segments against two, lengths spread 68 us
-// against 94, one long sequence 57-60 against 94, all full 109-112 against 96-99.
+// since sequences that all reach N lose by it: 4 x 4096, 16 heads of 64, four segments against two, lengths spread 66-86
+// us, one long sequence 64 and all full 121 against 94-109 for any.
 LdPlan ld_tc_plan(int64_t B, int64_t N, int64_t H, int64_t D, bool ragged, int* npart) {
   const int64_t units = B * H, slots = (int64_t)sm_count() * (D <= 32 ? 2 : 1), chunks = ceil_div(N, LT_C);
   auto segment = [&](int64_t len, int64_t real) -> int64_t {  // tenths of a chunk

@@ -50,3 +50,29 @@ def test_scores_keep_their_bits(N, D, relu):
 @pytest.mark.parametrize("D", [32, 64, 112, 128])
 def test_shared_heads_and_padded_batches(D):
     check(4, 113, 6, 2, D, True, [113, 0, 1, 70])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("D", [16, 48, 64])
+@pytest.mark.parametrize("N", [1, 64, 65, 128])
+def test_the_carried_state_keeps_its_bits(N, D, relu):
+    """Keys without features: an output is the state that came in times q.  Two bf16 terms of the state 2^-17 of the sum of the
+    absolute products, D truncated fp32 sums of two products each 2^-15, the power 2^-21: 2^-14 together, and half a step
+    (2^-8) of the result.  (Widths without room for a second term: see the header.)"""
+    B, H = 2, 5
+    g = torch.Generator().manual_seed(N + 7 * D + relu)
+    q = torch.randn(B * N, H * D, generator=g).bfloat16()
+    v = torch.randn(B * N, H * D, generator=g).bfloat16()
+    prior = torch.randn(B, H, D + 1, D, generator=g)
+    log_decay = -torch.linspace(0, 0.02, H)
+    out, state = ops.la_decay(q.cuda(), torch.zeros_like(q).cuda(), v.cuda(), log_decay.cuda(), B, N, H, D, scale=1.0, relu=relu,
+                              prior=prior.cuda())
+    f = q.double().view(B, N, H, D)
+    f = f.clamp(min=0) if relu else f
+    power = torch.exp(log_decay.double() * torch.arange(1, N + 1)[:, None])[None, :, :, None]
+    want = torch.einsum("bthd,bhed->bthe", f, prior[:, :, :D].double()) * power
+    mag = torch.einsum("bthd,bhed->bthe", f.abs(), prior[:, :, :D].double().abs()) * power
+    bound = 2.0 ** -14 * mag + 2.0 ** -8 * want.abs() + 1e-30
+    worst = ((out.double().cpu().view(B, N, H, D) - want).abs() / bound).max().item()
+    assert worst <= 1, f"{worst:.2f} times the bound"
