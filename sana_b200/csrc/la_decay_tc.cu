@@ -29,7 +29,7 @@
 // rate would allow 45); 8 x 4096 tokens, 70 heads of 32 246-254 us (2.4 TB/s; 90); 8 x 4096 tokens, 16 heads of 128 288 us
 // (two launches; 83); 4 x up to 4096, 16 heads of 64 over 8 of k and v 63-86.  What bounds it is the length of a chunk's
 // chain - copy, transform, products, join, state operand, products, output, each behind a barrier and with one warp per
-// scheduler for each role: the tensor pipe is busy 17-22 % of the time and DRAM 25-38 %.  Chunks of 128 halve the number of
+// scheduler for each role: the tensor pipe is busy 20-27 % of the time and DRAM 25-38 %.  Chunks of 128 halve the number of
 // chains that 64 would have, and two CTAs of narrow heads per SM overlap theirs; wide heads fill shared memory alone.
 // Single-lane waits (half the speed of converged ones) and roles that poll several barriers in turn were tried and were
 // slower.
